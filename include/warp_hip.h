@@ -2,7 +2,7 @@
  * warp_hip.h — C ABI of the MI355X (gfx950) backend for WARP's routed-expert
  * MoE path. Plain C, plain pointers and sizes.
  *
- * Two halves:
+ * Three parts:
  *
  *  1. The reference's dispatch table (src/waste_backend.h:67-94) and a
  *     registration function in its style (src/waste_backend.h:116-120,
@@ -15,6 +15,10 @@
  *     (vq_apply :2264, moe_layer :2713, moe_chunk :3512); these entry points
  *     replace them behind a context that keeps the codebooks, routers,
  *     shared experts and an expert cache resident in HBM.
+ *
+ *  3. Operators around a layer's recurrence and experts, for callers that
+ *     keep the rows in device memory: the short causal convolution, a
+ *     selective scan, tokens sorted by expert and brought back.
  *
  * Device pointers are named *_dev and live in the memory of the context's
  * device; everything else is host memory borrowed for the duration of the
@@ -556,6 +560,163 @@ int warp_hip_vq_encode_dev_noalloc(const float *X_dev, long n, const float *book
  * reference); returns the number of non-empty clusters, or a negative
  * WARP_HIP_E_* code. entries <= 4096. */
 int warp_hip_vq_lloyd(const float *X, int n, float *C, int entries, int dim, int nthreads);
+
+/* ---- 3. operators around a layer's recurrence and experts ------------------
+ *
+ * For callers that keep a layer's rows in device memory: the short causal
+ * convolution in front of a recurrence (warp_hip_kda_forward's q, k and v, or
+ * the scan below), a selective state space scan, and tokens sorted by expert
+ * for experts that the caller computes itself from warp_hip_route's picks.
+ * They take no context. Each queues its work on `stream` (a hipStream_t, NULL
+ * for the current device's null stream) and returns: nothing waits, allocates
+ * or copies, so every call can be captured into a graph. Buffers lie in the
+ * memory of the stream's device. Workspaces are the caller's: calls that may
+ * overlap (on two streams, or from two graphs) need one each.
+ *
+ * Rows are of one of three types, sums and states are f32. A row stride (ld*)
+ * is in elements, 0 for the rows' width. Buffers need their elements'
+ * alignment only. At most 2^24 channels. An output may not overlap an input, but where it says so.
+ * A call that is refused (WARP_HIP_E_ARG) has queued nothing. No counterpart
+ * in the reference but where it says so. */
+enum { WARP_HIP_F32 = 0, WARP_HIP_BF16 = 1, WARP_HIP_F16 = 2 };
+
+/* Rows of several sequences, for the convolution and the scan.
+ * Prompts: `tokens` rows hold n_seq sequences one after the other, sequence s
+ * in rows starts[s] .. starts[s + 1] - 1 (starts: n_seq + 1 ascending numbers
+ * within 0 .. tokens, in device memory; a sequence may be empty, its state is
+ * then carried over). Rows before the first and behind the last are left as
+ * they were. Single tokens: starts NULL and n_seq = tokens, row s is the next
+ * token of sequence s.
+ * Carried states lie in n_slots slots: sequence s reads its first state from
+ * slot slots[s] of state_in and leaves its last one there in state_out (slots
+ * NULL: slot s, n_slots >= n_seq). A sequence whose slot is not within 0 ..
+ * n_slots - 1 (-1: a padding row) is not computed: its rows and states stay
+ * as they were. Slots must differ: of two sequences with one slot, neither's
+ * results are defined. state_in NULL: zeros; state_out NULL: not wanted;
+ * state_out may be state_in, but overlap it in no other way. */
+
+/* y[t][c] = act(bias[c] + sum_j w[c][j] u[t - taps + 1 + j][c]), u a
+ * sequence's rows with its taps - 1 carried ones before them; act SiLU or
+ * none. A state is the last taps - 1 rows of u, [taps - 1][channels], the
+ * oldest first, of the rows' type (the reference's short_conv_step,
+ * src/waste_backend.h:73-74, keeps a ring for one token's step). */
+typedef struct {
+    int type;                     /* WARP_HIP_F32, _BF16 or _F16: x, y, states */
+    int tokens, n_seq, channels;
+    int taps;                     /* 1 .. 8                                  */
+    const int *starts, *slots;
+    int n_slots;
+    const void *x;                /* [tokens][channels]                      */
+    size_t ldx;
+    const float *w;               /* [channels][taps]                        */
+    const float *bias;            /* [channels] or NULL                      */
+    int silu;
+    const void *state_in;         /* [n_slots][taps - 1][channels]           */
+    void *state_out;
+    void *y;                      /* [tokens][channels]                      */
+    size_t ldy;
+} warp_hip_conv_args;
+int warp_hip_short_conv(const warp_hip_conv_args *a, void *stream);
+
+/* Per channel d of group g = d / (channels / groups), with states n:
+ *   dt' = softplus(dt + dt_bias), or dt + dt_bias
+ *   h[n] = exp(dt' A[d][n]) h[n] + dt' x B[g][n]
+ *   y    = (sum_n C[g][n] h[n] + D[d] x) silu(z)
+ * `longest` is the longest sequence's length where the caller knows it (0:
+ * not): it chooses how the work is split, results hold for any. Prompts need
+ * warp_hip_selective_scan_work() bytes of workspace, 16-byte aligned (0: none). */
+typedef struct {
+    int type;                     /* of x, dt, B, C, z, y                    */
+    int tokens, n_seq, channels;
+    int states;                   /* 1 .. 256                                */
+    int groups;                   /* divides channels                        */
+    const int *starts, *slots;
+    int n_slots;
+    const void *x;                /* [tokens][channels]                      */
+    size_t ldx;
+    const void *dt;               /* [tokens][channels]                      */
+    size_t lddt;
+    const float *A;               /* [channels][states]                      */
+    const void *B, *C;            /* [tokens][groups][states], one stride    */
+    size_t ldbc;
+    const float *D;               /* [channels] or NULL                      */
+    const void *z;                /* [tokens][channels] or NULL: no gate     */
+    size_t ldz;
+    const float *dt_bias;         /* [channels] or NULL                      */
+    int softplus;
+    const float *state_in;        /* [n_slots][channels][states]             */
+    float *state_out;
+    void *y;                      /* [tokens][channels]                      */
+    size_t ldy;
+    int longest;
+    void *work;
+    size_t work_bytes;
+} warp_hip_scan_args;
+int warp_hip_selective_scan(const warp_hip_scan_args *a, void *stream);
+size_t warp_hip_selective_scan_work(int tokens, int channels, int states, int n_seq, int longest);
+
+/* Sorts the pairs (t, k) of idx [tokens][top_k] by expert, in their own order
+ * within an expert. offsets [n_experts + 1]: where each expert's pairs begin,
+ * then how many there are; perm[p] = t * top_k + k of the pair at place p;
+ * pos[t][k] = p, or -1 where idx[t][k] is not within 0 .. n_experts - 1 (a
+ * padding token, an expert held elsewhere): such pairs have no place. With x,
+ * row p of xs [tokens * top_k][hidden] is a copy of row t of x. Places behind
+ * offsets[n_experts] are left as they were, in perm and in xs. n_experts <=
+ * 2048, tokens * top_k below 2^31 - 2048. Needs warp_hip_expert_dispatch_work()
+ * bytes of workspace, 4-byte aligned. The gradient of x is
+ * warp_hip_expert_combine without weights, of the gradient of xs. */
+typedef struct {
+    int tokens, top_k, n_experts;
+    const int *idx;
+    int *offsets, *perm, *pos;
+    int type;                     /* of x and xs                             */
+    int hidden;
+    const void *x;                /* [tokens][hidden], or NULL: no rows      */
+    size_t ldx;
+    void *xs;
+    size_t ldxs;
+    void *work;
+    size_t work_bytes;
+} warp_hip_dispatch_args;
+int warp_hip_expert_dispatch(const warp_hip_dispatch_args *a, void *stream);
+size_t warp_hip_expert_dispatch_work(int tokens, int top_k, int n_experts);
+
+/* out[t] = resid[t] + sum_k w[t][k] y[pos[t][k]], added in the order of k;
+ * pairs whose pos is not within 0 .. tokens * top_k - 1 add nothing. w NULL:
+ * weights of 1; resid NULL: none; out may be resid, at the same stride. */
+typedef struct {
+    int type;                     /* of y, resid, out                        */
+    int tokens, top_k, hidden;
+    const void *y;                /* [tokens * top_k][hidden]                */
+    size_t ldy;
+    const int *pos;               /* [tokens][top_k]                         */
+    const float *w;               /* [tokens][top_k] or NULL                 */
+    const void *resid;            /* [tokens][hidden] or NULL                */
+    size_t ldr;
+    void *out;                    /* [tokens][hidden]                        */
+    size_t ldo;
+} warp_hip_combine_args;
+int warp_hip_expert_combine(const warp_hip_combine_args *a, void *stream);
+
+/* The gradients of warp_hip_expert_combine: dy[pos[t][k]] = w[t][k] dout[t]
+ * and dw[t][k] = <dout[t], y[pos[t][k]]> (0 where the pair has no place; rows
+ * of dy that no pair names are left as they were). The residual's is dout.
+ * dy or dw may be NULL: not wanted (y is then only read for dw); dy may be y,
+ * at the same stride. No two pairs may name one place. */
+typedef struct {
+    int type;                     /* of dout, y, dy                          */
+    int tokens, top_k, hidden;
+    const void *dout;             /* [tokens][hidden]                        */
+    size_t ldd;
+    const void *y;                /* [tokens * top_k][hidden]                */
+    size_t ldy;
+    const int *pos;               /* [tokens][top_k]                         */
+    const float *w;               /* [tokens][top_k] or NULL                 */
+    void *dy;                     /* [tokens * top_k][hidden] or NULL        */
+    size_t lddy;
+    float *dw;                    /* [tokens][top_k] or NULL                 */
+} warp_hip_combine_back_args;
+int warp_hip_expert_combine_backward(const warp_hip_combine_back_args *a, void *stream);
 
 #ifdef __cplusplus
 }

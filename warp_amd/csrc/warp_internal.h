@@ -22,6 +22,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "warp_hip.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -413,6 +415,16 @@ int wk_crc32(const uint8_t *p, size_t n, uint32_t *tmp, uint32_t *out, const uin
  * 150 KiB. */
 int wk_kda(int T, int H, int K, int V, const float *q, const float *k, const float *v, const float *g,
            const float *beta, float *S, float *o, void *stream);
+
+/* The operators on packed rows (conv.hip, scan.hip, dispatch.hip), their
+ * arguments checked and their strides filled in. 0, or not. */
+int wk_short_conv(const warp_hip_conv_args *a, void *stream);
+int wk_selective_scan(const warp_hip_scan_args *a, void *stream);
+size_t wk_scan_work(int tokens, int channels, int states, int n_seq, int longest);
+int wk_expert_dispatch(const warp_hip_dispatch_args *a, void *stream);
+size_t wk_dispatch_work(int tokens, int top_k, int n_experts);
+int wk_expert_combine(const warp_hip_combine_args *a, void *stream);
+int wk_expert_combine_backward(const warp_hip_combine_back_args *a, void *stream);
 
 /* Device properties the host needs: returns the gfx name into buf. */
 int wk_device_arch(int device, char *buf, int n);

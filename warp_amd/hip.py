@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(HERE, "libwarp_hip.so")
 VQ3R, VQ2R, VQ4P, VQ12 = 4, 5, 8, 9
 FMT = {"VQ3R": VQ3R, "VQ2R": VQ2R, "VQ4P": VQ4P, "VQ12": VQ12}
 ROUTE_SIGMOID, ROUTE_SOFTMAX = 0, 1
+F32, BF16, F16 = 0, 1, 2
 ERRORS = {-1: "E_ARG", -2: "E_DEVICE", -3: "E_NOMEM", -4: "E_READ", -5: "E_HEADER",
           -6: "E_CRC", -7: "E_NOSLOT", -8: "E_MISSING", -9: "E_BOOKS"}
 E_ARG, E_DEVICE, E_NOMEM, E_READ, E_HEADER, E_CRC, E_NOSLOT, E_MISSING, E_BOOKS = range(-1, -10, -1)
@@ -87,6 +88,58 @@ class MoeKernels(C.Structure):
     """waste_moe_kernels: the MoE slots' table."""
     _fields_ = [("moe_ffn_decode", MOE_SLOT), ("moe_ffn_batch", MOE_SLOT), ("on_device", C.c_int)]
 
+
+class ConvArgs(C.Structure):
+    """warp_hip_conv_args"""
+    _fields_ = [
+        ("type", C.c_int), ("tokens", C.c_int), ("n_seq", C.c_int), ("channels", C.c_int), ("taps", C.c_int),
+        ("starts", C.c_void_p), ("slots", C.c_void_p), ("n_slots", C.c_int), ("x", C.c_void_p), ("ldx", C.c_size_t),
+        ("w", C.c_void_p), ("bias", C.c_void_p), ("silu", C.c_int), ("state_in", C.c_void_p),
+        ("state_out", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_size_t),
+    ]
+
+
+class ScanArgs(C.Structure):
+    """warp_hip_scan_args"""
+    _fields_ = [
+        ("type", C.c_int), ("tokens", C.c_int), ("n_seq", C.c_int), ("channels", C.c_int), ("states", C.c_int),
+        ("groups", C.c_int), ("starts", C.c_void_p), ("slots", C.c_void_p), ("n_slots", C.c_int),
+        ("x", C.c_void_p), ("ldx", C.c_size_t), ("dt", C.c_void_p), ("lddt", C.c_size_t), ("A", C.c_void_p),
+        ("B", C.c_void_p), ("C", C.c_void_p), ("ldbc", C.c_size_t), ("D", C.c_void_p), ("z", C.c_void_p),
+        ("ldz", C.c_size_t), ("dt_bias", C.c_void_p), ("softplus", C.c_int), ("state_in", C.c_void_p),
+        ("state_out", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_size_t), ("longest", C.c_int),
+        ("work", C.c_void_p), ("work_bytes", C.c_size_t),
+    ]
+
+
+class DispatchArgs(C.Structure):
+    """warp_hip_dispatch_args"""
+    _fields_ = [
+        ("tokens", C.c_int), ("top_k", C.c_int), ("n_experts", C.c_int), ("idx", C.c_void_p),
+        ("offsets", C.c_void_p), ("perm", C.c_void_p), ("pos", C.c_void_p), ("type", C.c_int), ("hidden", C.c_int),
+        ("x", C.c_void_p), ("ldx", C.c_size_t), ("xs", C.c_void_p), ("ldxs", C.c_size_t), ("work", C.c_void_p),
+        ("work_bytes", C.c_size_t),
+    ]
+
+
+class CombineArgs(C.Structure):
+    """warp_hip_combine_args"""
+    _fields_ = [
+        ("type", C.c_int), ("tokens", C.c_int), ("top_k", C.c_int), ("hidden", C.c_int), ("y", C.c_void_p),
+        ("ldy", C.c_size_t), ("pos", C.c_void_p), ("w", C.c_void_p), ("resid", C.c_void_p), ("ldr", C.c_size_t),
+        ("out", C.c_void_p), ("ldo", C.c_size_t),
+    ]
+
+
+class CombineBackArgs(C.Structure):
+    """warp_hip_combine_back_args"""
+    _fields_ = [
+        ("type", C.c_int), ("tokens", C.c_int), ("top_k", C.c_int), ("hidden", C.c_int), ("dout", C.c_void_p),
+        ("ldd", C.c_size_t), ("y", C.c_void_p), ("ldy", C.c_size_t), ("pos", C.c_void_p), ("w", C.c_void_p),
+        ("dy", C.c_void_p), ("lddy", C.c_size_t), ("dw", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); also the list of symbols the header declares
 SIGNATURES = {
     "waste_register_hip": (C.c_char_p, [C.c_void_p]),
@@ -154,6 +207,13 @@ SIGNATURES = {
     "warp_hip_vq_lloyd": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "warp_hip_vq_encode_dev_noalloc": (C.c_int, [C.c_void_p, C.c_long, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
                                                  C.c_void_p]),
+    "warp_hip_short_conv": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
+    "warp_hip_selective_scan": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),
+    "warp_hip_selective_scan_work": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "warp_hip_expert_dispatch": (C.c_int, [C.POINTER(DispatchArgs), C.c_void_p]),
+    "warp_hip_expert_dispatch_work": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "warp_hip_expert_combine": (C.c_int, [C.POINTER(CombineArgs), C.c_void_p]),
+    "warp_hip_expert_combine_backward": (C.c_int, [C.POINTER(CombineBackArgs), C.c_void_p]),
 }
 
 
@@ -472,6 +532,67 @@ def vq_lloyd(X, C):
     assert C.dtype == np.float32 and C.flags.c_contiguous
     return _check_rc(lib().warp_hip_vq_lloyd(X.ctypes.data, X.shape[0], C.ctypes.data, C.shape[0], C.shape[1], 0),
                      "vq_lloyd")
+
+
+# ---- operators around a layer's recurrence and experts (section 3 of the
+# header, which says what each computes). Buffers are device buffers or their
+# addresses, `dtype` is F32, BF16 or F16, row strides (ld*) are in elements
+# (0: the rows' width), `stream` a hipStream_t. A refused call raises.
+
+def short_conv(x, w, y, *, dtype, tokens, channels, taps, n_seq, n_slots, starts=None, slots=None, state_in=None,
+               state_out=None, bias=None, silu=True, ldx=0, ldy=0, stream=None):
+    """Short causal convolution over packed prompts (starts [n_seq + 1]) or
+    one token of each sequence (starts None)."""
+    a = ConvArgs(dtype, tokens, n_seq, channels, taps, _addr(starts), _addr(slots), n_slots, _addr(x), ldx, _addr(w),
+                 _addr(bias), silu, _addr(state_in), _addr(state_out), _addr(y), ldy)
+    _check_rc(lib().warp_hip_short_conv(a, stream), "short_conv")
+
+
+def selective_scan(x, dt, A, B, C, y, *, dtype, tokens, channels, n_state, n_seq, n_slots, groups=1, starts=None,
+                   slots=None, state_in=None, state_out=None, D=None, z=None, dt_bias=None, softplus=True, ldx=0,
+                   lddt=0, ldbc=0, ldz=0, ldy=0, longest=0, work=None, work_bytes=0, stream=None):
+    """Selective state space scan over packed prompts (starts [n_seq + 1],
+    with selective_scan_work() bytes of workspace) or one token of each
+    sequence (starts None)."""
+    a = ScanArgs(dtype, tokens, n_seq, channels, n_state, groups, _addr(starts), _addr(slots), n_slots, _addr(x), ldx,
+                 _addr(dt), lddt, _addr(A), _addr(B), _addr(C), ldbc, _addr(D), _addr(z), ldz, _addr(dt_bias), softplus,
+                 _addr(state_in), _addr(state_out), _addr(y), ldy, longest, _addr(work), work_bytes)
+    _check_rc(lib().warp_hip_selective_scan(a, stream), "selective_scan")
+
+
+def selective_scan_work(tokens, channels, n_state, n_seq, longest=0):
+    """Bytes of workspace that selective_scan needs for prompts of these sizes."""
+    return lib().warp_hip_selective_scan_work(tokens, channels, n_state, n_seq, longest)
+
+
+def expert_dispatch(idx, offsets, perm, pos, *, tokens, top_k, n_experts, x=None, xs=None, dtype=F32, hidden=0, ldx=0,
+                    ldxs=0, work=None, work_bytes=0, stream=None):
+    """Pairs (token, k) of idx [tokens][top_k] sorted by expert, and with x
+    their rows in xs; with expert_dispatch_work() bytes of workspace."""
+    a = DispatchArgs(tokens, top_k, n_experts, _addr(idx), _addr(offsets), _addr(perm), _addr(pos), dtype, hidden,
+                     _addr(x), ldx, _addr(xs), ldxs, _addr(work), work_bytes)
+    _check_rc(lib().warp_hip_expert_dispatch(a, stream), "expert_dispatch")
+
+
+def expert_dispatch_work(tokens, top_k, n_experts):
+    """Bytes of workspace that expert_dispatch needs."""
+    return lib().warp_hip_expert_dispatch_work(tokens, top_k, n_experts)
+
+
+def expert_combine(y, pos, out, *, dtype, tokens, top_k, hidden, w=None, resid=None, ldy=0, ldr=0, ldo=0, stream=None):
+    """The experts' rows back to their tokens: out = resid + sum_k w y[pos].
+    Without w, of xs's gradient, it is the gradient of expert_dispatch's x."""
+    a = CombineArgs(dtype, tokens, top_k, hidden, _addr(y), ldy, _addr(pos), _addr(w), _addr(resid), ldr, _addr(out), ldo)
+    _check_rc(lib().warp_hip_expert_combine(a, stream), "expert_combine")
+
+
+def expert_combine_backward(dout, y, pos, dy, dw, *, dtype, tokens, top_k, hidden, w=None, ldd=0, ldy=0, lddy=0,
+                            stream=None):
+    """Gradients of expert_combine: dy[pos] = w dout, dw = <dout, y[pos]>
+    (either may be None)."""
+    a = CombineBackArgs(dtype, tokens, top_k, hidden, _addr(dout), ldd, _addr(y), ldy, _addr(pos), _addr(w), _addr(dy),
+                        lddy, _addr(dw))
+    _check_rc(lib().warp_hip_expert_combine_backward(a, stream), "expert_combine_backward")
 
 
 def load_container_model(ctx: Context, model, layers=None, records=True):
