@@ -6,7 +6,10 @@
 // prompts too, and the carried rows lie in time order.
 //
 // What bounds it is memory: each input is read once, each output written
-// once, 2 taps + 4 operations on the vector units between them.
+// once, about 19 issue slots of the vector units between them (four taps, and
+// SiLU's two instructions at a quarter of the rate), half of the time memory
+// takes. 8,191 bf16 rows of 4,640 channels in 11 sequences: 35.6 us, 4.3 TB/s
+// (a copy of that size reaches 4.7); 46 us with stores that go through L2.
 
 #include "rows.h"
 #include "warp_internal.h"
@@ -14,7 +17,7 @@
 constexpr int CONV_MAX_TAPS = 8;
 
 struct conv_p {
-    int tokens, n_seq, C, taps, n_slots, run, silu;
+    int tokens, n_seq, C, taps, n_slots, run, silu;              // run: rows of a wave
     const int *starts, *slots;
     const void *x;
     size_t ldx;
@@ -26,33 +29,40 @@ struct conv_p {
 
 // A thread's V channels: weights and bias in registers, taps aligned to the
 // end of the window (KS = 0: any number of taps up to CONV_MAX_TAPS).
-template <typename T, int V, int KS>
+template <typename T, int KS, bool ONE>
 struct conv_t {
-    static constexpr int NT = KS ? KS : CONV_MAX_TAPS;
+    static constexpr int V = rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS;
     float w[NT][V], b[V];
     int first;                                    // of the window's NT places that hold a tap
     bool silu;
 
-    __device__ __forceinline__ void weights(const conv_p &p, int c0, int n) {
+    __device__ __forceinline__ conv_t(const conv_p &p, const cols_t<T, ONE> &k) {
         first = KS ? 0 : NT - p.taps;
         silu = p.silu;
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            b[i] = i < n && p.bias ? p.bias[c0 + i] : 0.0f;
+            b[i] = (!ONE || i < k.n) && p.bias ? p.bias[k.c + i] : 0.0f;
 #pragma unroll
             for (int j = 0; j < NT; j++)
-                w[j][i] = i < n && j >= first ? p.w[(size_t)(c0 + i) * (NT - first) + j - first] : 0.0f;
+                w[j][i] = (!ONE || i < k.n) && (KS || j >= first) ? p.w[(size_t)(k.c + i) * (NT - first) + j - first]
+                                                                  : 0.0f;
         }
     }
-    // u[first .. NT - 1]: the inputs, the newest last
-    __device__ __forceinline__ vec_t<T, V> out(const vec_t<T, V> *u) const {
+    // A row's outputs, from the window u[first .. NT - 2] before it; the
+    // window moves on by the row.
+    __device__ __forceinline__ vec_t<T, V> step(float (&u)[NT][V], const vec_t<T, V> &x) const {
         vec_t<T, V> y;
 #pragma unroll
         for (int i = 0; i < V; i++) {
+            const float c = (float)x.e[i];
             float a = b[i];
 #pragma unroll
-            for (int j = 0; j < NT; j++)
-                if (KS || j >= first) a = __builtin_fmaf(w[j][i], (float)u[j].e[i], a);
+            for (int j = 0; j < NT - 1; j++)
+                if (KS || j >= first) a = __builtin_fmaf(w[j][i], u[j][i], a);
+            a = __builtin_fmaf(w[NT - 1][i], c, a);
+#pragma unroll
+            for (int j = 0; j + 1 < NT - 1; j++) u[j][i] = u[j + 1][i];
+            if (NT > 1) u[NT - 2][i] = c;
             y.e[i] = (T)(silu ? rows_silu(a) : a);
         }
         return y;
@@ -60,120 +70,141 @@ struct conv_t {
 };
 
 // One token of each of n_seq sequences: a thread takes V channels of one.
-template <typename T, int KS>
+template <typename T, int KS, bool ONE>
 __global__ __launch_bounds__(256) void k_conv_token(conv_p p) {
     constexpr int V = rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS;
-    const int c0 = ((int)blockIdx.x * (int)blockDim.x + (int)threadIdx.x) * V, n = min(V, p.C - c0);
-    if (n <= 0) return;
-    conv_t<T, V, KS> k;
-    k.weights(p, c0, n);
-    const int hist = NT - 1 - k.first;
+    const int c0 = ((int)blockIdx.x * (int)blockDim.x + (int)threadIdx.x) * V;
+    if (c0 >= p.C) return;
+    const cols_t<T, ONE> k(c0, p.C);
+    const conv_t<T, KS, ONE> conv(p, k);
+    const int hist = NT - 1 - conv.first;
     for (int s = blockIdx.y; s < p.n_seq; s += gridDim.y) {
         const int slot = seq_slot(p.slots, s, p.n_slots);
         if (slot < 0) continue;
-        vec_t<T, V> u[NT];
-        const T *in = (const T *)p.sin + (size_t)slot * hist * p.C + c0;
+        vec_t<T, V> h[NT], x = k.load((const T *)p.x + (size_t)s * p.ldx + k.c);
+        const T *in = (const T *)p.sin + (size_t)slot * hist * p.C + k.c;
+        float u[NT][V];
+#pragma unroll
+        for (int j = 0; j < NT - 1; j++) {
+            h[j].e = 0;
+            if (p.sin && (KS || j >= conv.first)) h[j] = k.load(in + (size_t)(j - conv.first) * p.C);
+        }
+        h[NT - 1] = x;
 #pragma unroll
         for (int j = 0; j < NT - 1; j++)
-            if (KS || j >= k.first) u[j] = load_vec<T, V>(in + (size_t)(j - k.first) * p.C, p.sin ? n : 0);
-        u[NT - 1] = load_vec<T, V>((const T *)p.x + (size_t)s * p.ldx + c0, n);
-        store_vec<T, V>((T *)p.y + (size_t)s * p.ldy + c0, k.out(u), n);
+#pragma unroll
+            for (int i = 0; i < V; i++) u[j][i] = (float)h[j].e[i];
+        k.store((T *)p.y + (size_t)s * p.ldy + k.c, conv.step(u, x));
         if (!p.sout) continue;
-        T *out = (T *)p.sout + (size_t)slot * hist * p.C + c0;
+        T *out = (T *)p.sout + (size_t)slot * hist * p.C + k.c;
 #pragma unroll
         for (int j = 0; j < NT - 1; j++)
-            if (KS || j >= k.first) store_vec<T, V>(out + (size_t)(j - k.first) * p.C, u[j + 1], n);
+            if (KS || j >= conv.first) k.store(out + (size_t)(j - conv.first) * p.C, h[j + 1]);
     }
 }
 
 // Packed sequences: a wave takes 64 V channels of a run of rows, whatever
 // sequences the run holds, so that ragged batches split evenly. The window
 // slides through registers, so a run reads its own rows once and taps - 1
-// before it.
+// before it; the next rows are loaded while these are computed.
 // A sequence's first taps - 1 rows (those that read the carried inputs) all
 // belong to the run in which the sequence begins, past that run's end if
 // need be; the same thread then writes the inputs to carry on. So state_out
-// may be state_in: nobody else reads a slot's state.
-template <typename T, int KS>
+// may be state_in: what a thread uses of a slot's state nobody else writes.
+template <typename T, int KS, bool ONE>
 __global__ __launch_bounds__(256) void k_conv_rows(conv_p p) {
     constexpr int V = rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS, U = 4;
+    typedef vec_t<T, V> vec;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int c0 = ((int)blockIdx.x * 64 + lane) * V, n = min(V, p.C - c0);
-    if (n <= 0) return;
-    conv_t<T, V, KS> k;
-    k.weights(p, c0, n);
-    const int hist = NT - 1 - k.first, runs = max(1, (p.tokens + p.run - 1) / p.run);
-    const T *x = (const T *)p.x + c0;
-    T *y = (T *)p.y + c0;
+    const int c0 = ((int)blockIdx.x * 64 + lane) * V, runs = max(1, (p.tokens + p.run - 1) / p.run);
+    const seqs_t seqs(p.starts, p.slots, p.n_seq, p.tokens, p.n_slots);
+    const bool live = c0 < p.C;
+    const cols_t<T, ONE> k(live ? c0 : p.C - 1, p.C);
+    const conv_t<T, KS, ONE> conv(p, k);
+    const int hist = NT - 1 - conv.first;
+    const T *x = (const T *)p.x + k.c;
+    T *y = (T *)p.y + k.c;
     for (int q = (int)blockIdx.y * 4 + wave; q < runs; q += (int)gridDim.y * 4) {
-        const int r0 = q * p.run, r1 = min(r0 + p.run, p.tokens);
-        for (int s = seq_from(p.starts, p.n_seq, r0); s < p.n_seq; s++) {
-            const seq_t seq = seq_at(p.starts, s, p.tokens);
+        const int r0 = q * p.run, r1 = min(r0 + p.run, p.tokens), s0 = seqs.from(r0);
+        if (!live) continue;
+        for (int s = s0; s < p.n_seq; s++) {
+            const seq_t seq = seqs.at(s);
             if (seq.b >= r1 && q + 1 < runs) break;
             const bool mine = seq.b >= r0;        // it begins here
-            const int slot = seq_slot(p.slots, s, p.n_slots);
-            if (slot < 0) continue;
-            const T *in = p.sin ? (const T *)p.sin + (size_t)slot * hist * p.C + c0 : nullptr;
+            if (seq.slot < 0) continue;
+            const T *in = p.sin ? (const T *)p.sin + (size_t)seq.slot * hist * p.C + k.c : nullptr;
+            // row t of the sequence, or of the inputs carried to it
+            auto before = [&](int t) {
+                vec v;
+                v.e = 0;
+                if (t >= seq.b) v = k.load(x + (size_t)t * p.ldx);
+                else if (in) v = k.load(in + (size_t)(hist + t - seq.b) * p.C);
+                return v;
+            };
             const int lo = mine ? seq.b : max(r0, seq.b + hist), hi = min(seq.e, mine ? max(r1, seq.b + hist) : r1);
             if (lo < hi) {
-                vec_t<T, V> u[NT - 1 + U], nx[U];
+                float u[NT][V];
+                vec cu[U], nx[U];
 #pragma unroll
-                for (int i = 0; i < U; i++) nx[i] = load_vec<T, V>(x + (size_t)(lo + i) * p.ldx, lo + i < hi ? n : 0);
+                for (int i = 0; i < U; i++) nx[i] = k.load(x + (size_t)min(lo + i, hi - 1) * p.ldx);
 #pragma unroll
                 for (int j = 0; j < NT - 1; j++) {
-                    const int at = lo - (NT - 1) + j;
-                    if (!KS && j < k.first) continue;
-                    if (at >= seq.b) u[j] = load_vec<T, V>(x + (size_t)at * p.ldx, n);
-                    else u[j] = load_vec<T, V>(in + (ptrdiff_t)(hist + at - seq.b) * p.C, in ? n : 0);
+                    if (!KS && j < conv.first) continue;
+                    const vec v = before(lo - (NT - 1) + j);
+#pragma unroll
+                    for (int i = 0; i < V; i++) u[j][i] = (float)v.e[i];
                 }
                 for (int t = lo; t < hi; t += U) {
 #pragma unroll
-                    for (int i = 0; i < U; i++) u[NT - 1 + i] = nx[i];
+                    for (int i = 0; i < U; i++) cu[i] = nx[i];
+                    if (t + U < hi) {
+#pragma unroll
+                        for (int i = 0; i < U; i++) nx[i] = k.load(x + (size_t)min(t + U + i, hi - 1) * p.ldx);
+                    }
 #pragma unroll
                     for (int i = 0; i < U; i++)
-                        nx[i] = load_vec<T, V>(x + (size_t)(t + U + i) * p.ldx, t + U + i < hi ? n : 0);
-#pragma unroll
-                    for (int i = 0; i < U; i++)
-                        if (t + i < hi) store_vec<T, V>(y + (size_t)(t + i) * p.ldy, k.out(u + i), n);
-#pragma unroll
-                    for (int j = 0; j < NT - 1; j++) u[j] = u[j + U];
+                        if (t + i < hi) k.stream(y + (size_t)(t + i) * p.ldy, conv.step(u, cu[i]));
                 }
             }
             if (!mine || !p.sout) continue;
-            T *out = (T *)p.sout + (size_t)slot * hist * p.C + c0;
+            T *out = (T *)p.sout + (size_t)seq.slot * hist * p.C + k.c;
             // in ascending order, which state_out = state_in allows: a row
             // moves to its own place or one before it
-            for (int j = 0; j < hist; j++) {
-                const int at = seq.e - hist + j;
-                const vec_t<T, V> v = at >= seq.b ? load_vec<T, V>(x + (size_t)at * p.ldx, n)
-                                                  : load_vec<T, V>(in + (ptrdiff_t)(hist + at - seq.b) * p.C, in ? n : 0);
-                store_vec<T, V>(out + (size_t)j * p.C, v, n);
-            }
+            for (int j = 0; j < hist; j++) k.store(out + (size_t)j * p.C, before(seq.e - hist + j));
         }
     }
 }
 
-template <typename T>
-static void conv_launch(const conv_p &p, bool token, hipStream_t st) {
+template <typename T, int KS, bool ONE>
+static void conv_launch(conv_p p, hipStream_t st) {
     constexpr int V = rows_of<T>::V;
-    const int groups = (p.C + V - 1) / V;
-    if (token) {
-        const dim3 grid((groups + 63) / 64, p.n_seq < 32768 ? p.n_seq : 32768), block(64);
-        if (p.taps == 4) hipLaunchKernelGGL((k_conv_token<T, 4>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((k_conv_token<T, 0>), grid, block, 0, st, p);
+    const int cols = ((p.C + V - 1) / V + 63) / 64;
+    if (!p.starts) {
+        hipLaunchKernelGGL((k_conv_token<T, KS, ONE>), dim3(cols, p.n_seq < 32768 ? p.n_seq : 32768), dim3(64), 0, st, p);
         return;
     }
-    const int runs = (p.tokens + p.run - 1) / p.run, blocks = runs < 4 ? 1 : (runs + 3) / 4;
-    const dim3 grid((groups + 63) / 64, blocks < 32768 ? blocks : 32768), block(256);
-    if (p.taps == 4) hipLaunchKernelGGL((k_conv_rows<T, 4>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((k_conv_rows<T, 0>), grid, block, 0, st, p);
+    // Runs of 16 rows read 3 of 19 twice and load their weights once, but a
+    // batch has to make enough waves of them: 7,000 rows of 1,024 channels take
+    // 13.8, 13.2 and 15.6 us in runs of 16, 8 and 4, 1,000 rows of 513 take 18.2,
+    // 11.6 and 7.8, the 8,191 of 4,640 below 35.6, 39.2 and 55.3.
+    const int64_t work = (int64_t)p.tokens * cols;
+    p.run = work >= 16 * 768 ? 16 : work >= 8 * 768 ? 8 : 4;
+    const int blocks = (p.tokens + 4 * p.run - 1) / (4 * p.run);
+    hipLaunchKernelGGL((k_conv_rows<T, KS, ONE>), dim3(cols, blocks < 1 ? 1 : blocks < 32768 ? blocks : 32768), dim3(256), 0,
+                       st, p);
+}
+template <typename T>
+static void conv_type(const conv_p &p, hipStream_t st) {
+    if (p.C < rows_of<T>::V) conv_launch<T, 0, true>(p, st);
+    else if (p.taps == 4) conv_launch<T, 4, false>(p, st);
+    else conv_launch<T, 0, false>(p, st);
 }
 
 extern "C" int wk_short_conv(const warp_hip_conv_args *a, void *stream) {
     conv_p p = {a->tokens, a->n_seq, a->channels, a->taps, a->n_slots, 16, a->silu, a->starts, a->slots, a->x, a->ldx,
                 a->w, a->bias, a->state_in, a->state_out, a->y, a->ldy};
-    if (a->type == WARP_HIP_F32) conv_launch<float>(p, !a->starts, (hipStream_t)stream);
-    else if (a->type == WARP_HIP_BF16) conv_launch<bf16_t>(p, !a->starts, (hipStream_t)stream);
-    else conv_launch<f16_t>(p, !a->starts, (hipStream_t)stream);
+    if (a->type == WARP_HIP_F32) conv_type<float>(p, (hipStream_t)stream);
+    else if (a->type == WARP_HIP_BF16) conv_type<bf16_t>(p, (hipStream_t)stream);
+    else conv_type<f16_t>(p, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

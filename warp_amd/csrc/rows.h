@@ -44,7 +44,46 @@ struct rows_of<f16_t> {
     static constexpr int V = 8;
 };
 
-// n of V elements (the last vector of a row may be short; the rest are 0)
+// A thread's vector of a row of C elements. Where C is no multiple of V the
+// last thread's begins early, at C - V, so that it loads a whole vector too,
+// and it stores only what no other thread has: its elements from `skip` on.
+// ONE: rows shorter than a vector, element by element.
+template <typename T, bool ONE>
+struct cols_t {
+    static constexpr int V = rows_of<T>::V;
+    typedef vec_t<T, V> vec;
+    int c, skip, n;                               // its first column; see above; elements there are
+
+    __device__ __forceinline__ cols_t(int c0, int C) : c(ONE ? c0 : min(c0, C - V)), skip(c0 - c), n(min(V, C - c)) {}
+    __device__ __forceinline__ vec load(const T *p) const {
+        vec v;
+        if (!ONE) {
+            v.e = *(const typename vec::mem *)p;
+            return v;
+        }
+        v.e = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) v.e[i] = p[i];
+        return v;
+    }
+    __device__ __forceinline__ void part(T *p, const vec &v) const {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i >= skip && i < n) p[i] = v.e[i];
+    }
+    __device__ __forceinline__ void store(T *p, const vec &v) const {
+        if (!ONE && skip == 0) *(typename vec::mem *)p = v.e;
+        else part(p, v);
+    }
+    // The same past the caches, for outputs that are larger than those: what
+    // they would push out of L2 is worth more.
+    __device__ __forceinline__ void stream(T *p, const vec &v) const {
+        if (!ONE && skip == 0) __builtin_nontemporal_store(v.e, (typename vec::mem *)p);
+        else part(p, v);
+    }
+};
+// n of V elements (0 where there are none)
 template <typename T, int V>
 __device__ __forceinline__ vec_t<T, V> load_vec(const T *p, int n) {
     vec_t<T, V> v;
@@ -52,7 +91,9 @@ __device__ __forceinline__ vec_t<T, V> load_vec(const T *p, int n) {
     if (n >= V) {
         v.e = *(const typename vec_t<T, V>::mem *)p;
     } else if (n > 0) {
-        for (int i = 0; i < n; i++) v.e[i] = p[i];
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) v.e[i] = p[i];
     }
     return v;
 }
@@ -61,7 +102,9 @@ __device__ __forceinline__ void store_vec(T *p, const vec_t<T, V> &v, int n) {
     if (n >= V) {
         *(typename vec_t<T, V>::mem *)p = v.e;
     } else if (n > 0) {
-        for (int i = 0; i < n; i++) p[i] = v.e[i];
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < n) p[i] = v.e[i];
     }
 }
 
@@ -71,26 +114,61 @@ __device__ __forceinline__ void store_vec(T *p, const vec_t<T, V> &v, int n) {
 __device__ __forceinline__ float rows_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 __device__ __forceinline__ float rows_silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + rows_exp(-x)); }
 
-// Where sequence s of a packed batch begins and ends: starts[s] and
-// starts[s + 1], kept within the rows there are.
+// The sequences of a packed batch: sequence s holds the rows b .. e - 1,
+// starts[s] and starts[s + 1] kept within the rows there are, and its state
+// is in a slot (-1: in none, its rows are not computed). A wave loads up to 63
+// sequences at once, a lane each, so that finding one and walking on from it
+// costs one trip to memory; of more it searches 64 at a time.
 struct seq_t {
-    int b, e;
+    int b, e, slot;
 };
-__device__ __forceinline__ seq_t seq_at(const int *__restrict__ starts, int s, int tokens) {
-    const int b = min(max(starts[s], 0), tokens), e = min(max(starts[s + 1], 0), tokens);
-    return {b, max(b, e)};
-}
-// the first sequence that does not end before row t (n_seq if all do)
-__device__ __forceinline__ int seq_from(const int *__restrict__ starts, int n_seq, int t) {
-    int lo = 0, hi = n_seq;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid + 1] >= t) hi = mid;
-        else lo = mid + 1;
+struct seqs_t {
+    const int *starts, *slots;
+    int n, tokens, n_slots, lane, b, e, k;
+    bool few;
+
+    // (all 64 lanes take part here and in from())
+    __device__ __forceinline__ seqs_t(const int *st, const int *sl, int n_seq, int rows, int ns)
+        : starts(st), slots(sl), n(n_seq), tokens(rows), n_slots(ns), lane(threadIdx.x & 63), few(n_seq < 64) {
+        const int i = min(lane, n - 1);
+        b = few ? starts[i] : 0;
+        e = few ? starts[i + 1] : 0;
+        k = few && slots ? slots[i] : i;
     }
-    return lo;
-}
-// the slot of sequence s's state; -1: none, its rows are not computed
+    // the first sequence that does not end before row t (n if all do)
+    __device__ __forceinline__ int from(int t) const {
+        if (few) {
+            const uint64_t m = __ballot(lane < n && e >= t);
+            return m ? __builtin_ctzll(m) : n;
+        }
+        int lo = 0, hi = n;                       // it is in lo .. hi
+        while (hi > lo) {
+            const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
+            const uint64_t m = __ballot(i < hi && starts[min(i, n - 1) + 1] < t);
+            const int c = __popcll(m);            // that many of the samples are before it
+            if (c == 0) return lo;
+            lo += (c - 1) * step + 1;
+            hi = min(hi, lo + step - 1);
+        }
+        return lo;
+    }
+    __device__ __forceinline__ seq_t at(int s) const {
+        int vb, ve, vk;
+        if (few) {
+            vb = __builtin_amdgcn_readlane(b, s);
+            ve = __builtin_amdgcn_readlane(e, s);
+            vk = __builtin_amdgcn_readlane(k, s);
+        } else {
+            vb = starts[s];
+            ve = starts[s + 1];
+            vk = slots ? slots[s] : s;
+        }
+        vb = min(max(vb, 0), tokens);
+        ve = min(max(ve, 0), tokens);
+        return {vb, max(vb, ve), (unsigned)vk < (unsigned)n_slots ? vk : -1};
+    }
+};
+// one token of each sequence: its slot
 __device__ __forceinline__ int seq_slot(const int *__restrict__ slots, int s, int n_slots) {
     const int k = slots ? slots[s] : s;
     return (unsigned)k < (unsigned)n_slots ? k : -1;

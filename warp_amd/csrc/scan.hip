@@ -211,26 +211,23 @@ __global__ __launch_bounds__(64) void k_scan_rows(scan_p p) {
     k.open(p);
     const size_t dn = (size_t)p.D * p.N;
     const int units = p.chunk ? p.chunks : p.n_seq;
+    const seqs_t seqs(p.starts, p.slots, p.n_seq, p.tokens, p.n_slots);
     for (int j = blockIdx.y; j < units; j += gridDim.y) {
-        int r0 = 0, r1 = p.tokens, s = j;
-        if (p.chunk) {
-            r0 = j * p.chunk;
-            r1 = min(r0 + p.chunk, p.tokens);
-            s = seq_from(p.starts, p.n_seq, r0);
-        }
-        for (; s < p.n_seq; s++) {
-            const seq_t q = seq_at(p.starts, s, p.tokens);
+        const int r0 = j * p.chunk, r1 = p.chunk ? min(r0 + p.chunk, p.tokens) : p.tokens;
+        for (int s = p.chunk ? seqs.from(r0) : j; s < p.n_seq; s++) {
+            const seq_t q = seqs.at(s);
             if (p.chunk && q.b >= r1 && j + 1 < units) break;
-            const int slot = seq_slot(p.slots, s, p.n_slots);
-            if (slot >= 0 && (q.b >= r0 || q.e > r0)) {
+            if (q.slot >= 0 && (q.b >= r0 || q.e > r0)) {
                 // (a sequence that goes on past its chunk has its first state
                 // in `init`: its last state may be in the same slot already)
                 const bool past = p.chunk && q.e > r1;
                 const float *from = q.b < r0 ? p.end + (size_t)(j - 1) * dn
-                                             : !p.sin ? nullptr : past ? p.init + (size_t)j * dn : p.sin + (size_t)slot * dn;
+                                    : !p.sin ? nullptr
+                                    : past   ? p.init + (size_t)j * dn
+                                             : p.sin + (size_t)q.slot * dn;
                 k.state(p, from);
                 k.template rows<true>(p, max(q.b, r0), min(q.e, r1), bc);
-                if (!past && p.sout) k.store(p, p.sout + (size_t)slot * dn);
+                if (!past && p.sout) k.store(p, p.sout + (size_t)q.slot * dn);
             }
             if (!p.chunk) break;
         }
@@ -247,15 +244,15 @@ __global__ __launch_bounds__(64) void k_scan_part(scan_p p) {
     scan_t<T, S, LPC, U> k;
     k.open(p);
     const size_t dn = (size_t)p.D * p.N;
+    const seqs_t seqs(p.starts, p.slots, p.n_seq, p.tokens, p.n_slots);
     for (int j = blockIdx.y; j + 1 < p.chunks; j += gridDim.y) {
         const int r0 = j * p.chunk, r1 = r0 + p.chunk;
         // the sequence that row r1 belongs to, if it holds row r1 - 1 too
-        const int s = seq_from(p.starts, p.n_seq, r1 + 1);
-        const seq_t q = s < p.n_seq ? seq_at(p.starts, s, p.tokens) : seq_t{r1, r1};
-        const int slot = q.b < r1 ? seq_slot(p.slots, s, p.n_slots) : -1;
-        if (slot < 0) continue;
+        const int s = seqs.from(r1 + 1);
+        const seq_t q = s < p.n_seq ? seqs.at(s) : seq_t{r1, r1, -1};
+        if (q.slot < 0 || q.b >= r1) continue;
         const bool begins = q.b >= r0;
-        const float *from = begins && p.sin ? p.sin + (size_t)slot * dn : nullptr;
+        const float *from = begins && p.sin ? p.sin + (size_t)q.slot * dn : nullptr;
         k.state(p, from);
         if (from) k.store(p, p.init + (size_t)j * dn);
         const float sum = k.template rows<false>(p, max(q.b, r0), r1, bc);
