@@ -107,6 +107,12 @@ __device__ __forceinline__ void store_vec(T *p, const vec_t<T, V> &v, int n) {
             if (i < n) p[i] = v.e[i];
     }
 }
+// (past the caches, as above)
+template <typename T, int V>
+__device__ __forceinline__ void stream_vec(T *p, const vec_t<T, V> &v, int n) {
+    if (n >= V) __builtin_nontemporal_store(v.e, (typename vec_t<T, V>::mem *)p);
+    else store_vec<T, V>(p, v, n);
+}
 
 // exp and the sigmoid on the exponential instruction (2^x within an ulp; the
 // product with log2 e adds |x| 2^-24 of relative error, which only matters

@@ -7,11 +7,13 @@
 // to end, dt' and the sums too; only x, dt, B, C, z and y are of the rows' type.
 //
 // What bounds prompts is the vector units: per row, channel and state a
-// product and an exponential for the decay (the exponential issues at a
-// quarter of the rate), a product, and two fused multiply-adds, about eight
-// issue slots, against 8 bytes of rows per channel. The decays differ by
-// channel and state, so nothing of this is a matrix product. Single tokens
-// are bound by their states, read and written once.
+// product and an exponential for the decay (the exponential issues at half
+// the rate), a product, and two fused multiply-adds, six issue slots, against
+// 8 bytes of rows per channel. The decays differ by channel and state, so
+// nothing of this is a matrix product. Single tokens are bound by their
+// states, read and written once.
+
+#include <math.h>
 
 #include "rows.h"
 #include "warp_internal.h"
@@ -58,44 +60,38 @@ __device__ __forceinline__ float scan_sum(float v) {
 }
 
 // One token of each of n_seq sequences. LPC lanes share a channel, W states
-// each in a run (their state row is read and written 4 W bytes a lane), and
-// keep that channel's decay rates for the rows of sequences they take in turn.
+// each in a run (of rows that are no whole number of runs the last is short),
+// and keep that channel's decay rates for the sequences they take in turn.
+// 256 sequences of 4,608 channels by 16 states, bf16: 31.1 us, 5.2 TB/s (a
+// copy that leaves the caches behind reaches 4.7); 44 us with stores through
+// L2. Single states (W = 1) for rows that are no multiple of 4 take 69 us for
+// 200 sequences of 3,000 by 23, these 57.
 template <typename T, int W, int LPC>
 __global__ __launch_bounds__(256) void k_scan_token(scan_p p) {
-    constexpr int NI = W == 1 && LPC == 64 ? 4 : 1;        // (64 lanes of single states take them in up to four turns)
     const int lane = threadIdx.x % LPC, d = ((int)blockIdx.x * 256 + (int)threadIdx.x) / LPC;
     if (d >= p.D) return;
-    const int n0 = lane * W, g = d / (p.D / p.G);
-    float A[NI][W];
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-        const int n = n0 + i * LPC * W;
-        const vec_t<float, W> a = load_vec<float, W>(p.A + (size_t)d * p.N + n, p.N - n);
-#pragma unroll
-        for (int j = 0; j < W; j++) A[i][j] = a.e[j] * LOG2E;
-    }
+    const int n = lane * W, m = p.N - n, g = d / (p.D / p.G);
+    vec_t<float, W> A = load_vec<float, W>(p.A + (size_t)d * p.N + n, m);
+    A.e *= LOG2E;
     const float bias = p.bias ? p.bias[d] : 0.0f, skip = p.skip ? p.skip[d] : 0.0f;
     for (int s = blockIdx.y; s < p.n_seq; s += gridDim.y) {
         const int slot = seq_slot(p.slots, s, p.n_slots);
         if (slot < 0) continue;
+        const size_t at = ((size_t)slot * p.D + d) * p.N + n, bc = (size_t)s * p.ldbc + (size_t)g * p.N + n;
+        vec_t<float, W> h = load_vec<float, W>(p.sin + at, p.sin ? m : 0);
+        const vec_t<T, W> B = load_vec<T, W>((const T *)p.B + bc, m), C = load_vec<T, W>((const T *)p.C + bc, m);
         const float x = (float)((const T *)p.x)[(size_t)s * p.ldx + d];
-        float dt = (float)((const T *)p.dt)[(size_t)s * p.lddt + d] + bias;
-        if (p.softplus) dt = scan_softplus(dt);
-        const size_t at = ((size_t)slot * p.D + d) * p.N, bc = (size_t)s * p.ldbc + (size_t)g * p.N;
-        const float u = dt * x;
+        float v = (float)((const T *)p.dt)[(size_t)s * p.lddt + d] + bias;
+        if (p.softplus) v = scan_softplus(v);
+        const float u = v * x;
         float y = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int n = n0 + i * LPC * W, m = p.N - n;
-            const vec_t<T, W> B = load_vec<T, W>((const T *)p.B + bc + n, m), C = load_vec<T, W>((const T *)p.C + bc + n, m);
-            vec_t<float, W> h = load_vec<float, W>(p.sin + at + n, p.sin ? m : 0);
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-                h.e[j] = __builtin_fmaf(h.e[j], __builtin_amdgcn_exp2f(dt * A[i][j]), u * (float)B.e[j]);
-                y = __builtin_fmaf(h.e[j], j < m ? (float)C.e[j] : 0.0f, y);
-            }
-            if (p.sout) store_vec<float, W>(p.sout + at + n, h, m);
+        for (int j = 0; j < W; j++) {
+            h.e[j] = __builtin_fmaf(h.e[j], __builtin_amdgcn_exp2f(v * A.e[j]), u * (float)B.e[j]);
+            y = __builtin_fmaf(h.e[j], (float)C.e[j], y);
         }
+        // (past L2: by the next token the other layers' states have been through it)
+        if (p.sout) stream_vec<float, W>(p.sout + at, h, m);
         y = scan_sum<LPC>(y);
         y = __builtin_fmaf(skip, x, y);
         if (p.z) y *= rows_silu((float)((const T *)p.z)[(size_t)s * p.ldz + d]);
@@ -104,98 +100,156 @@ __global__ __launch_bounds__(256) void k_scan_token(scan_p p) {
 }
 
 // Prompts. LPC lanes of a wave share a channel, S states each in registers;
-// a wave is a block and takes 64 / LPC channels of one group. A batch of U
-// rows' B and C is laid out in LDS as f32, where all lanes read the same
-// address; x, dt and z go to registers a batch ahead.
+// a wave is a block and takes 64 / LPC channels of one group. The rows go in
+// batches of U: their B and C are laid out in LDS as f32, where a row's lie at
+// one address for all channels; x, dt and z go to registers. All are loaded a
+// batch ahead. A full batch is one straight run of instructions (the states'
+// chain of multiply-adds is the only thing that waits, S of them in turn).
 template <typename T, int S, int LPC, int U>
 struct scan_t {
     static constexpr int RS = S * LPC;                     // states, filled up
     float A[S], h[S], bias, skip;
     int lane, part, d, g;
-    bool live;
 
+    // (a wave's spare lanes repeat its last channel, and store what that does)
     __device__ __forceinline__ void open(const scan_p &p) {
         const int per = p.D / p.G, blocks = (per * LPC + 63) / 64, i = (int)blockIdx.x % blocks;
         lane = threadIdx.x;
         part = lane % LPC;
         g = (int)blockIdx.x / blocks;
-        const int c = (i * 64 + lane) / LPC;
-        live = c < per;
-        d = g * per + min(c, per - 1);                     // (a wave's spare lanes repeat the last channel)
-#pragma unroll
-        for (int n = 0; n < S; n++) A[n] = part * S + n < p.N ? p.A[(size_t)d * p.N + part * S + n] * LOG2E : 0.0f;
+        d = g * per + min((i * 64 + lane) / LPC, per - 1);
         bias = p.bias ? p.bias[d] : 0.0f;
         skip = p.skip ? p.skip[d] : 0.0f;
-    }
-    __device__ __forceinline__ void state(const scan_p &p, const float *at) {
+        get(p, A, p.A);
 #pragma unroll
-        for (int n = 0; n < S; n++)
-            h[n] = at && part * S + n < p.N ? at[(size_t)d * p.N + part * S + n] : 0.0f;
+        for (int n = 0; n < S; n++) A[n] *= LOG2E;
     }
-    __device__ __forceinline__ void store(const scan_p &p, float *at) const {
+    // This lane's states' values of an array [D][N] (0 where it has none), four
+    // at a time if the rows are whole fours: the lanes' are a row apart, and
+    // each instruction costs a look into a cache line per lane.
+    __device__ __forceinline__ void get(const scan_p &p, float (&v)[S], const float *from) const {
+        const float *at = from + (size_t)d * p.N + part * S;
+        const int m = p.N - part * S;
+        if (p.N % 4 == 0) {
 #pragma unroll
-        for (int n = 0; n < S; n++)
-            if (live && part * S + n < p.N) at[(size_t)d * p.N + part * S + n] = h[n];
+            for (int n = 0; n < S; n += 4) {
+                const vec_t<float, 4> q = load_vec<float, 4>(at + n, n < m ? 4 : 0);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[n + i] = q.e[i];
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < S; n++) v[n] = n < m ? at[n] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void state(const scan_p &p, const float *from) {
+        if (from) {
+            get(p, h, from);
+        } else {
+#pragma unroll
+            for (int n = 0; n < S; n++) h[n] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ void store(const scan_p &p, float *to) const {
+        float *at = to + (size_t)d * p.N + part * S;
+        const int m = p.N - part * S;
+        if (p.N % 4 == 0) {
+#pragma unroll
+            for (int n = 0; n < S; n += 4) {
+                vec_t<float, 4> q;
+#pragma unroll
+                for (int i = 0; i < 4; i++) q.e[i] = h[n + i];
+                if (n < m) store_vec<float, 4>(at + n, q, 4);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < S; n++)
+                if (n < m) at[n] = h[n];
+        }
     }
 
-    // Rows lo .. hi of one sequence. OUT: with y; without, dt' is summed up.
+    // Rows lo .. hi - 1 of one sequence. OUT: with y; without, dt' is summed up.
     template <bool OUT>
     __device__ __forceinline__ float rows(const scan_p &p, int lo, int hi, float *bc) {
-        constexpr int K = OUT ? 2 : 1;                     // B, or B and C
-        constexpr int M = (U * K * RS + 63) / 64;
+        constexpr int K = OUT ? 2 : 1, M = (U * K * RS + 63) / 64;       // B, or B and C
         if (lo >= hi) return 0.0f;
-        float tx[U], td[U], tz[U], tb[M], sum = 0.0f;
-        const T *x = (const T *)p.x + d, *dt = (const T *)p.dt + d, *z = (const T *)p.z + d;
-        const T *B = (const T *)p.B + (size_t)g * p.N, *C = (const T *)p.C + (size_t)g * p.N;
+        T tx[U], td[U], tz[U], tb[M];
+        float sum = 0.0f;
+        const unsigned at = d * sizeof(T);
         auto load = [&](int t) {
 #pragma unroll
             for (int i = 0; i < U; i++) {
                 const size_t r = min(t + i, hi - 1);
-                tx[i] = (float)x[r * p.ldx];
-                td[i] = (float)dt[r * p.lddt];
-                if (OUT && p.z) tz[i] = (float)z[r * p.ldz];
+                tx[i] = *(const T *)((const char *)((const T *)p.x + r * p.ldx) + at);
+                td[i] = *(const T *)((const char *)((const T *)p.dt + r * p.lddt) + at);
+                if (OUT && p.z) tz[i] = *(const T *)((const char *)((const T *)p.z + r * p.ldz) + at);
             }
 #pragma unroll
             for (int i = 0; i < M; i++) {
-                const int e = lane + 64 * i, n = e % RS, k = e / RS % K;
-                const size_t r = min(t + e / (RS * K), hi - 1);
-                tb[i] = n < p.N ? (float)(k ? C : B)[r * p.ldbc + n] : 0.0f;
+                const int e = lane + 64 * i, n = min(e % RS, p.N - 1), r = min(e / (RS * K), hi - 1 - t);
+                const T *row = (const T *)(OUT && e / RS % K ? p.C : p.B) + (size_t)t * p.ldbc + (size_t)g * p.N;
+                tb[i] = row[(size_t)r * p.ldbc + n];
             }
         };
         load(lo);
         for (int t = lo; t < hi; t += U) {
-            float cx[U], cd[U], cz[U];
-#pragma unroll
-            for (int i = 0; i < U; i++) cx[i] = tx[i], cd[i] = td[i], cz[i] = tz[i];
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < M; i++)
-                if (U * K * RS % 64 == 0 || lane + 64 * i < U * K * RS) bc[lane + 64 * i] = tb[i];
-            __syncthreads();                               // (one wave: its LDS writes are done)
-            if (t + U < hi) load(t + U);
+            float x[U], v[U], z[U], y[U];
 #pragma unroll
             for (int i = 0; i < U; i++) {
-                if (t + i >= hi) break;
-                float v = cd[i] + bias;
-                if (p.softplus) v = scan_softplus(v);
-                const float u = v * cx[i];
+                x[i] = (float)tx[i];
+                v[i] = (float)td[i] + bias;
+                if (OUT && p.z) z[i] = (float)tz[i];
+            }
+#pragma unroll
+            for (int i = 0; i < M; i++)
+                if (U * K * RS % 64 == 0 || lane + 64 * i < U * K * RS)
+                    bc[lane + 64 * i] = (lane + 64 * i) % RS < p.N ? (float)tb[i] : 0.0f;
+            // (one wave: what it writes to LDS is there for its next reads)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (t + U < hi) load(t + U);
+            if (p.softplus) {
+#pragma unroll
+                for (int i = 0; i < U; i++) v[i] = scan_softplus(v[i]);
+            }
+            auto row = [&](int i) {
+                const float u = v[i] * x[i];
                 const float *b = bc + i * K * RS + part * S, *c = b + RS;
-                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float o[4];
 #pragma unroll
                 for (int n = 0; n < S; n++) {
-                    h[n] = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(v * A[n]), u * b[n]);
-                    if (OUT) y[n & 3] = __builtin_fmaf(h[n], c[n], y[n & 3]);
+                    h[n] = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(v[i] * A[n]), u * b[n]);
+                    if (OUT) o[n & 3] = n < 4 ? h[n] * c[n] : __builtin_fmaf(h[n], c[n], o[n & 3]);
                 }
-                if (OUT) {
-                    float o = scan_sum<LPC>((y[0] + y[1]) + (y[2] + y[3]));
-                    o = __builtin_fmaf(skip, cx[i], o);
-                    if (p.z) o *= rows_silu(cz[i]);
-                    if (live && part == 0) ((T *)p.y)[(size_t)(t + i) * p.ldy + d] = (T)o;
-                } else {
-                    sum += v;
+                if (OUT) y[i] = scan_sum<LPC>((o[0] + o[1]) + (o[2] + o[3]));
+                else sum += v[i];
+            };
+            auto out = [&](int n) {
+#pragma unroll
+                for (int i = 0; i < U; i++) y[i] = __builtin_fmaf(skip, x[i], y[i]);
+                if (p.z) {
+#pragma unroll
+                    for (int i = 0; i < U; i++) y[i] *= rows_silu(z[i]);
                 }
+#pragma unroll
+                for (int i = 0; i < U; i++)
+                    if (n == U || i < n)
+                        *(T *)((char *)((T *)p.y + (size_t)(t + i) * p.ldy) + at) = (T)y[i];
+            };
+            if (t + U <= hi) {
+#pragma unroll
+                for (int i = 0; i < U; i++) row(i);
+                if (OUT) out(U);
+            } else {
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    y[i] = 0.0f;
+                    if (t + i < hi) row(i);
+                }
+                if (OUT) out(hi - t);
             }
-            __syncthreads();                               // the batch's rows are read
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
         return sum;
     }
@@ -257,45 +311,93 @@ __global__ __launch_bounds__(64) void k_scan_part(scan_p p) {
         if (from) k.store(p, p.init + (size_t)j * dn);
         const float sum = k.template rows<false>(p, max(q.b, r0), r1, bc);
         k.store(p, p.end + (size_t)j * dn);
-        if (k.live && k.part == 0) p.sum[(size_t)j * p.D + k.d] = sum;
+        if (k.part == 0) p.sum[(size_t)j * p.D + k.d] = sum;
         if (blockIdx.x == 0 && k.lane == 0) p.reset[j] = begins;
     }
 }
 
-// The chunks in order: end[j] becomes the state at the end of chunk j.
-__global__ __launch_bounds__(256) void k_scan_join(scan_p p) {
-    const size_t dn = (size_t)p.D * p.N, i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= dn) return;
-    const int d = (int)(i / p.N);
-    const float A = p.A[i] * LOG2E;
-    float h = 0.0f;
-    for (int j = 0; j + 1 < p.chunks; j++) {
-        const float e = p.end[(size_t)j * dn + i], s = p.sum[(size_t)j * p.D + d];
-        h = p.reset[j] ? e : __builtin_fmaf(h, __builtin_amdgcn_exp2f(A * s), e);
-        p.end[(size_t)j * dn + i] = h;
+// The chunks in order: end[j] becomes the state at the end of chunk j. A lane
+// takes one state, each of the block's waves a part of the chunks: first what
+// the part makes of a state of zero and how much it leaves of one, then, from
+// the state that the parts before it leave, the states themselves. Up to
+// JOIN_Q chunks of a part stay in registers between the two.
+constexpr int JOIN_Q = 12, JOIN_W = 16;
+__global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
+    __shared__ float sum[JOIN_W][64], left[JOIN_W][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const size_t dn = (size_t)p.D * p.N, i = (size_t)blockIdx.x * 64 + lane, at = min(i, dn - 1);
+    const int d = (int)(at / p.N), most = p.chunks - 1, q = (most + waves - 1) / waves;
+    const int j0 = min(wave * q, most), j1 = min(j0 + q, most);
+    const float A = p.A[at] * LOG2E;
+    float h = 0.0f, w = 1.0f, e[JOIN_Q], f[JOIN_Q];        // (-1: nothing of what was before is left)
+    auto load = [&](int j) {
+        int r[JOIN_Q];
+#pragma unroll
+        for (int b = 0; b < JOIN_Q; b++)
+            if (j + b < j1) {
+                e[b] = p.end[(size_t)(j + b) * dn + at];
+                f[b] = p.sum[(size_t)(j + b) * p.D + d];
+                r[b] = p.reset[j + b];
+            }
+#pragma unroll
+        for (int b = 0; b < JOIN_Q; b++)
+            if (j + b < j1) f[b] = r[b] ? -1.0f : __builtin_amdgcn_exp2f(A * f[b]);
+    };
+    auto walk = [&](int j, bool keep) {
+#pragma unroll
+        for (int b = 0; b < JOIN_Q; b++)
+            if (j + b < j1) {
+                h = f[b] < 0.0f ? e[b] : __builtin_fmaf(h, f[b], e[b]);
+                w = f[b] < 0.0f || w < 0.0f ? -1.0f : w * f[b];
+                if (keep && i < dn) p.end[(size_t)(j + b) * dn + at] = h;
+            }
+    };
+    for (int j = j0; j < j1; j += JOIN_Q) {
+        load(j);
+        if (waves > 1 || q > JOIN_Q) walk(j, waves == 1);
+    }
+    if (waves > 1) {
+        sum[wave][lane] = h;
+        left[wave][lane] = w;
+        __syncthreads();
+        h = 0.0f;
+        for (int v = 0; v < wave; v++) h = left[v][lane] < 0.0f ? sum[v][lane] : __builtin_fmaf(h, left[v][lane], sum[v][lane]);
+    }
+    if (q <= JOIN_Q) {
+        walk(j0, true);
+    } else if (waves > 1) {
+        for (int j = j0; j < j1; j += JOIN_Q) {
+            load(j);
+            walk(j, true);
+        }
     }
 }
 
-// The split of a packed batch of prompts: chunk = 0, a wave (per 64 / LPC
-// channels) for each sequence, or chunks of so many rows.
-// A wave's rows come one after the other, so that a batch is fast when its
-// longest sequence is short, or there are more waves than the 1,024 SIMDs hold
-// anyway. Chunks make waves at the price of computing the states twice.
+// The split of a packed batch of prompts: chunk = 0, a wave (per 64 / lanes
+// channels) for each sequence, or chunks of so many rows, whose states are
+// computed twice. Both sides' times as a model that fits what was measured:
+// one bf16 prompt of 4,096 rows, 4,608 channels and 16 states takes 1,800 us
+// as a sequence per wave and 177 us in 40 chunks (72 + 9 + 96); 13 sequences
+// of 1,999 rows with 2,304 channels and 64 states, the longest of about 400,
+// take 180 us and 166; 60 of about 100 rows each are faster by themselves.
 struct scan_plan {
     int lanes, chunk, chunks;
 };
 static scan_plan scan_split(int tokens, int D, int N, int n_seq, int longest) {
     scan_plan r = {1, 0, 0};
     while (r.lanes * 16 < N) r.lanes *= 2;
+    // ns of a row: of a wave by itself (memory's latency), and of one among
+    // as many as keep the SIMDs busy
     const double simds = 1024, waves = ((double)D * r.lanes + 63) / 64, states = N < 16 ? N : 16;
-    const double all = 8 * states + 45, part = 7 * states + 30;      // issue slots of a row
+    const double alone = 440, all = 14 * states + 112, part = 11 * states + 76;
+    const double rows = tokens * waves / simds;
     if (longest <= 0 || longest > tokens) longest = tokens;
-    double most = 2 * simds / waves;
-    if (most > tokens / 32) most = tokens / 32;
+    double most = 3 * simds / waves;              // three waves to a SIMD, as registers allow
+    if (most > tokens / 16) most = tokens / 16;
     if (most < 2) return r;
     const int chunk = ((int)(tokens / most) + 7) / 8 * 8, chunks = (tokens + chunk - 1) / chunk;
-    const double direct = all * (longest > tokens * waves / simds ? longest : tokens * waves / simds);
-    const double split = (all + part) * (chunk > tokens * waves / simds ? chunk : tokens * waves / simds) + 4000;
+    const double direct = fmax(alone * longest, all * rows);
+    const double split = fmax(alone * chunk, all * rows) + fmax(0.75 * alone * chunk, part * rows) + 15000;
     if (chunks >= 2 && split < direct) r.chunk = chunk, r.chunks = chunks;
     return r;
 }
@@ -309,13 +411,15 @@ static void scan_rows_launch(const scan_p &p, hipStream_t st) {
     auto rows = [](int n) { return (unsigned)(n < 32768 ? n : 32768); };
     if (p.chunk) {
         hipLaunchKernelGGL((k_scan_part<T, S, LPC, U>), dim3(blocks, rows(p.chunks - 1)), dim3(64), 0, st, p);
-        hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((size_t)p.D * p.N + 255) / 256)), dim3(256), 0, st, p);
+        const int parts = (p.chunks + JOIN_Q - 2) / JOIN_Q;
+        hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((size_t)p.D * p.N + 63) / 64)),
+                           dim3(64 * (parts < JOIN_W ? parts : JOIN_W)), 0, st, p);
     }
     hipLaunchKernelGGL((k_scan_rows<T, S, LPC, U>), dim3(blocks, rows(p.chunk ? p.chunks : p.n_seq)), dim3(64), 0, st, p);
 }
 template <typename T, int W, int LPC>
 static void scan_token_launch(const scan_p &p, hipStream_t st) {
-    const int blocks = (int)(((size_t)p.D * LPC + 255) / 256), most = 4096 / blocks + 1;
+    const int blocks = (int)(((size_t)p.D * LPC + 255) / 256), most = 9216 / blocks + 1;     // (36 blocks a CU: 32.6 us; 16: 33.2, a block a row: 34.9)
     hipLaunchKernelGGL((k_scan_token<T, W, LPC>), dim3(blocks, p.n_seq < most ? p.n_seq : most), dim3(256), 0, st, p);
 }
 
@@ -325,23 +429,20 @@ static void scan_launch(const scan_p &p, hipStream_t st) {
     if (p.starts) {
         if (N <= 4) scan_rows_launch<T, 4, 1, 8>(p, st);
         else if (N <= 8) scan_rows_launch<T, 8, 1, 8>(p, st);
-        else if (N <= 16) scan_rows_launch<T, 16, 1, 8>(p, st);
-        else if (N <= 32) scan_rows_launch<T, 16, 2, 8>(p, st);
-        else if (N <= 64) scan_rows_launch<T, 16, 4, 8>(p, st);
+        else if (N <= 16) scan_rows_launch<T, 16, 1, 4>(p, st);
+        else if (N <= 32) scan_rows_launch<T, 16, 2, 4>(p, st);
+        else if (N <= 64) scan_rows_launch<T, 16, 4, 4>(p, st);
         else if (N <= 128) scan_rows_launch<T, 16, 8, 4>(p, st);
         else scan_rows_launch<T, 16, 16, 2>(p, st);
-    } else if (N % 4 == 0) {
-        if (N <= 4) scan_token_launch<T, 4, 1>(p, st);
+    } else {
+        if (N < 4) scan_token_launch<T, 1, 4>(p, st);
+        else if (N == 4) scan_token_launch<T, 4, 1>(p, st);
         else if (N <= 8) scan_token_launch<T, 4, 2>(p, st);
         else if (N <= 16) scan_token_launch<T, 4, 4>(p, st);
         else if (N <= 32) scan_token_launch<T, 4, 8>(p, st);
         else if (N <= 64) scan_token_launch<T, 4, 16>(p, st);
         else if (N <= 128) scan_token_launch<T, 4, 32>(p, st);
         else scan_token_launch<T, 4, 64>(p, st);
-    } else {
-        if (N <= 8) scan_token_launch<T, 1, 8>(p, st);
-        else if (N <= 32) scan_token_launch<T, 1, 32>(p, st);
-        else scan_token_launch<T, 1, 64>(p, st);
     }
 }
 
