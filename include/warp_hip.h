@@ -575,7 +575,7 @@ int warp_hip_vq_lloyd(const float *X, int n, float *C, int entries, int dim, int
  *
  * Rows are of one of three types, sums and states are f32. A row stride (ld*)
  * is in elements, 0 for the rows' width. Buffers need their elements'
- * alignment only. At most 2^24 channels. An output may not overlap an input, but where it says so.
+ * alignment only. Rows are at most 2^24 wide. An output may not overlap an input, but where it says so.
  * A call that is refused (WARP_HIP_E_ARG) has queued nothing. No counterpart
  * in the reference but where it says so. */
 enum { WARP_HIP_F32 = 0, WARP_HIP_BF16 = 1, WARP_HIP_F16 = 2 };

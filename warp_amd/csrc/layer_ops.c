@@ -137,7 +137,7 @@ int warp_hip_expert_dispatch(const warp_hip_dispatch_args *args, void *stream)
     if (!a.x != !a.xs) return WARP_HIP_E_ARG;
     if (a.x) {
         const int es = type_size(a.type);
-        if (!es || a.hidden < 1 || a.hidden > INT_MAX - 4096 || off(a.x, es) || off(a.xs, es)) return WARP_HIP_E_ARG;
+        if (!es || a.hidden < 1 || a.hidden > MAX_CHANNELS || off(a.x, es) || off(a.xs, es)) return WARP_HIP_E_ARG;
         a.ldx = stride(a.ldx, (size_t)a.hidden);
         a.ldxs = stride(a.ldxs, (size_t)a.hidden);
         if (!a.ldx || !a.ldxs) return WARP_HIP_E_ARG;
@@ -152,7 +152,7 @@ int warp_hip_expert_combine(const warp_hip_combine_args *args, void *stream)
     if (!args) return WARP_HIP_E_ARG;
     warp_hip_combine_args a = *args;
     const int es = type_size(a.type);
-    if (!es || !pairs_ok(a.tokens, a.top_k) || a.hidden < 1 || a.hidden > INT_MAX - 4096) return WARP_HIP_E_ARG;
+    if (!es || !pairs_ok(a.tokens, a.top_k) || a.hidden < 1 || a.hidden > MAX_CHANNELS) return WARP_HIP_E_ARG;
     a.ldy = stride(a.ldy, (size_t)a.hidden);
     a.ldr = stride(a.ldr, (size_t)a.hidden);
     a.ldo = stride(a.ldo, (size_t)a.hidden);
@@ -168,7 +168,7 @@ int warp_hip_expert_combine_backward(const warp_hip_combine_back_args *args, voi
     if (!args) return WARP_HIP_E_ARG;
     warp_hip_combine_back_args a = *args;
     const int es = type_size(a.type);
-    if (!es || !pairs_ok(a.tokens, a.top_k) || a.hidden < 1 || a.hidden > INT_MAX - 4096) return WARP_HIP_E_ARG;
+    if (!es || !pairs_ok(a.tokens, a.top_k) || a.hidden < 1 || a.hidden > MAX_CHANNELS) return WARP_HIP_E_ARG;
     a.ldd = stride(a.ldd, (size_t)a.hidden);
     a.ldy = stride(a.ldy, (size_t)a.hidden);
     a.lddy = stride(a.lddy, (size_t)a.hidden);

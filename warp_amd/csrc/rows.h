@@ -67,6 +67,14 @@ struct cols_t {
             if (i < n) v.e[i] = p[i];
         return v;
     }
+    // The same of rows that nothing reads again: they take no one's place in
+    // the caches.
+    __device__ __forceinline__ vec take(const T *p) const {
+        if (ONE) return load(p);
+        vec v;
+        v.e = __builtin_nontemporal_load((const typename vec::mem *)p);
+        return v;
+    }
     __device__ __forceinline__ void part(T *p, const vec &v) const {
 #pragma unroll
         for (int i = 0; i < V; i++)
