@@ -575,7 +575,8 @@ int warp_hip_vq_lloyd(const float *X, int n, float *C, int entries, int dim, int
  *
  * Rows are of one of three types, sums and states are f32. A row stride (ld*)
  * is in elements, 0 for the rows' width. Buffers need their elements'
- * alignment only. Rows are at most 2^24 wide. An output may not overlap an input, but where it says so.
+ * alignment only. Rows are at most 2^24 wide, and there are at most 2^30
+ * of them (and of sequences). An output may not overlap an input, but where it says so.
  * A call that is refused (WARP_HIP_E_ARG) has queued nothing. No counterpart
  * in the reference but where it says so. */
 enum { WARP_HIP_F32 = 0, WARP_HIP_BF16 = 1, WARP_HIP_F16 = 2 };
@@ -662,7 +663,7 @@ size_t warp_hip_selective_scan_work(int tokens, int channels, int states, int n_
  * padding token, an expert held elsewhere): such pairs have no place. With x,
  * row p of xs [tokens * top_k][hidden] is a copy of row t of x. Places behind
  * offsets[n_experts] are left as they were, in perm and in xs. n_experts <=
- * 2048, tokens * top_k below 2^31 - 2048. Needs warp_hip_expert_dispatch_work()
+ * 2048, tokens * top_k <= 2^30. Needs warp_hip_expert_dispatch_work()
  * bytes of workspace, 4-byte aligned. The gradient of x is
  * warp_hip_expert_combine without weights, of the gradient of xs. */
 typedef struct {

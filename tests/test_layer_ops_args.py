@@ -42,7 +42,7 @@ def back():
 
 
 ROWS = [dict(type=3), dict(type=-1), dict(tokens=-1), dict(n_seq=-1), dict(channels=0), dict(channels=(1 << 24) + 1),
-        dict(tokens=2 ** 31 - 1), dict(n_slots=2), dict(n_slots=-1, slots=A), dict(starts=None), dict(starts=A + 2),
+        dict(tokens=(1 << 30) + 1), dict(n_seq=(1 << 30) + 1, slots=A), dict(n_slots=2), dict(n_slots=-1, slots=A), dict(starts=None), dict(starts=A + 2),
         dict(slots=A + 1), dict(ldx=7), dict(ldy=7), dict(x=None), dict(y=None), dict(x=A + 2), dict(y=A + 1),
         dict(state_in=A + 2), dict(state_out=A + 2), dict(type=1, x=A + 1)]
 
@@ -71,8 +71,9 @@ def test_scan_refuses_a_short_workspace():
 @pytest.mark.parametrize("change", [dict(tokens=-1), dict(top_k=0), dict(n_experts=0), dict(n_experts=2049), dict(idx=None),
                                     dict(offsets=None), dict(perm=None), dict(pos=None), dict(idx=A + 1), dict(offsets=A + 2),
                                     dict(perm=A + 3), dict(pos=A + 2), dict(x=None), dict(xs=None), dict(type=5),
-                                    dict(hidden=0), dict(hidden=2 ** 31 - 1), dict(ldx=15), dict(ldxs=15), dict(x=A + 2),
-                                    dict(xs=A + 1), dict(work=None), dict(work=A + 2), dict(work_bytes=4),
+                                    dict(hidden=0), dict(hidden=(1 << 24) + 1), dict(ldx=15), dict(ldxs=15), dict(x=A + 2),
+                                    dict(xs=A + 1), dict(tokens=2000, work=None), dict(tokens=2000, work=A + 2),
+                                    dict(tokens=2000, work_bytes=4), dict(tokens=(1 << 29) + 1),
                                     dict(tokens=1 << 30, top_k=2)])
 def test_dispatch_refuses(change):
     assert refused(wh.lib().warp_hip_expert_dispatch, dispatch(), **change) == wh.E_ARG

@@ -1,7 +1,6 @@
 /* The operators around a layer's recurrence and experts: what include/warp_hip.h
  * section 3 promises of their arguments, checked before anything is queued.
  * The kernels are in conv.hip, scan.hip and dispatch.hip. */
-#include <limits.h>
 #include <stdint.h>
 
 #include <hip/hip_runtime_api.h>
@@ -12,6 +11,7 @@
 #define CONV_MAX_TAPS 8
 #define SCAN_MAX_STATES 256
 #define MAX_CHANNELS (1 << 24)
+#define MAX_ROWS (1 << 30)       /* what the kernels count in ints, with room to step over the end */
 #define DISPATCH_MAX_EXPERTS 2048
 
 static int type_size(int type)
@@ -61,7 +61,7 @@ static size_t stride(size_t ld, size_t width)
 static int sequences_ok(int tokens, int n_seq, int channels, const int *starts, const int *slots, int n_slots)
 {
     if (tokens < 0 || n_seq < 0 || channels < 1 || n_slots < 0 || off(starts, 4) || off(slots, 4)) return 0;
-    if (tokens > INT_MAX - 4096 || channels > MAX_CHANNELS) return 0;
+    if (tokens > MAX_ROWS || n_seq > MAX_ROWS || channels > MAX_CHANNELS) return 0;
     if (!starts && n_seq != tokens) return 0;
     return slots || n_slots >= n_seq;
 }
@@ -118,7 +118,7 @@ int warp_hip_selective_scan(const warp_hip_scan_args *args, void *stream)
 /* tokens * top_k pairs, as the kernels count them */
 static int pairs_ok(int tokens, int top_k)
 {
-    return tokens >= 0 && top_k >= 1 && (int64_t)tokens * top_k < INT_MAX - 2048;
+    return tokens >= 0 && top_k >= 1 && (int64_t)tokens * top_k <= MAX_ROWS;
 }
 
 size_t warp_hip_expert_dispatch_work(int tokens, int top_k, int n_experts)

@@ -237,10 +237,12 @@ def _addr(x):
     """Address of a device buffer (torch tensor or int) or a numpy array."""
     if x is None:
         return None
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(type(x))
