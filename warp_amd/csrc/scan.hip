@@ -99,15 +99,46 @@ __global__ __launch_bounds__(256) void k_scan_token(scan_p p) {
     }
 }
 
+// What lane p of each group of LPC lanes has, in all of the group's lanes.
+template <int LPC>
+__device__ __forceinline__ float scan_from(float v, int p) {
+    const int x = __float_as_int(v);
+#define DPP(old, ctl, banks) __builtin_amdgcn_update_dpp(old, x, ctl, 0xf, banks, false)
+#define FROM(ctl) __int_as_float(__builtin_amdgcn_mov_dpp(x, ctl, 0xf, 0xf, true))
+    if (LPC == 1) return v;
+    if (LPC == 2) return p == 0 ? FROM(0xa0) : FROM(0xf5);                       // quad_perm
+    if (LPC == 4) return p == 0 ? FROM(0x00) : p == 1 ? FROM(0x55) : p == 2 ? FROM(0xaa) : FROM(0xff);
+    // a row's lane to the row; with two groups in a row, lane p to the banks of one and 8 + p to the other's
+#define ROW(n) (LPC == 16 ? FROM(0x150 + n) : __int_as_float(DPP(DPP(x, 0x150 + n, 0x3), 0x150 + ((n + 8) & 15), 0xc)))
+    switch (p) {
+    case 0: return ROW(0);
+    case 1: return ROW(1);
+    case 2: return ROW(2);
+    case 3: return ROW(3);
+    case 4: return ROW(4);
+    case 5: return ROW(5);
+    case 6: return ROW(6);
+    default: return ROW(7);
+    }
+#undef ROW
+#undef FROM
+#undef DPP
+}
+
 // Prompts. LPC lanes of a wave share a channel, S states each in registers;
 // a wave is a block and takes 64 / LPC channels of one group. The rows go in
 // batches of U: their B and C are laid out in LDS as f32, where a row's lie at
-// one address for all channels; x, dt and z go to registers. All are loaded a
-// batch ahead. A full batch is one straight run of instructions (the states'
-// chain of multiply-adds is the only thing that waits, S of them in turn).
+// one address for all channels. Of x, dt and z a lane takes the rows that are
+// its own among the group's (all of them, if it has the channel to itself):
+// loads them a batch ahead, makes dt' of them, hands that to the other lanes
+// row by row, and gates and stores their outputs. A full batch is one straight
+// run of instructions (the states' chain of multiply-adds is the only thing
+// that waits, S of them in turn).
 template <typename T, int S, int LPC, int U>
 struct scan_t {
     static constexpr int RS = S * LPC;                     // states, filled up
+    static constexpr int P = LPC < U ? LPC : U, R = U / P; // lanes of a group with rows of their own, rows each
+    static_assert(P <= 8 || LPC == 1, "scan_from hands on the first eight lanes' values");
     float A[S], h[S], bias, skip;
     int lane, part, d, g;
 
@@ -171,87 +202,113 @@ struct scan_t {
     // Rows lo .. hi - 1 of one sequence. OUT: with y; without, dt' is summed up.
     template <bool OUT>
     __device__ __forceinline__ float rows(const scan_p &p, int lo, int hi, float *bc) {
-        constexpr int K = OUT ? 2 : 1, M = (U * K * RS + 63) / 64;       // B, or B and C
+        // B, or B and C, by fours of states a lane where a row has more than 4, else one by one
+        constexpr int K = OUT ? 2 : 1, W = LPC > 1 ? 4 : 1, Q = U * K * RS / W, M = (Q + 63) / 64;
         if (lo >= hi) return 0.0f;
-        T tx[U], td[U], tz[U], tb[M];
+        T tx[R], td[R], tz[R];
+        vec_t<T, W> tb[M];
         float sum = 0.0f;
         const unsigned at = d * sizeof(T);
+        const int own = part % P;                          // this lane's rows: own, own + P, ...
         auto load = [&](int t) {
 #pragma unroll
-            for (int i = 0; i < U; i++) {
-                const size_t r = min(t + i, hi - 1);
+            for (int i = 0; i < R; i++) {
+                const size_t r = min(t + i * P + (P > 1 ? own : 0), hi - 1);
                 tx[i] = *(const T *)((const char *)((const T *)p.x + r * p.ldx) + at);
                 td[i] = *(const T *)((const char *)((const T *)p.dt + r * p.lddt) + at);
                 if (OUT && p.z) tz[i] = *(const T *)((const char *)((const T *)p.z + r * p.ldz) + at);
             }
 #pragma unroll
             for (int i = 0; i < M; i++) {
-                const int e = lane + 64 * i, n = min(e % RS, p.N - 1), r = min(e / (RS * K), hi - 1 - t);
+                const int e = (lane + 64 * i) * W, n = e % RS, r = min(e / (RS * K), hi - 1 - t);
                 const T *row = (const T *)(OUT && e / RS % K ? p.C : p.B) + (size_t)t * p.ldbc + (size_t)g * p.N;
-                tb[i] = row[(size_t)r * p.ldbc + n];
+                // (the last of a row's begins early, as not to pass its end)
+                tb[i].e = *(const typename vec_t<T, W>::mem *)(row + (size_t)r * p.ldbc + min(n, p.N - W));
             }
         };
         load(lo);
         for (int t = lo; t < hi; t += U) {
-            float x[U], v[U], z[U], y[U];
+            float x[R], v[R], u[R], z[R], y[R];
 #pragma unroll
-            for (int i = 0; i < U; i++) {
+            for (int i = 0; i < R; i++) {
                 x[i] = (float)tx[i];
                 v[i] = (float)td[i] + bias;
                 if (OUT && p.z) z[i] = (float)tz[i];
             }
 #pragma unroll
-            for (int i = 0; i < M; i++)
-                if (U * K * RS % 64 == 0 || lane + 64 * i < U * K * RS)
-                    bc[lane + 64 * i] = (lane + 64 * i) % RS < p.N ? (float)tb[i] : 0.0f;
+            for (int i = 0; i < M; i++) {
+                const int e = (lane + 64 * i) * W, n = e % RS, skip = n + W - p.N;
+                vec_t<float, W> w;
+#pragma unroll
+                for (int j = 0; j < W; j++) w.e[j] = n < p.N ? (float)tb[i].e[j] : 0.0f;
+                if (W > 1 && p.N % W && skip > 0) {
+                    const auto all = w.e;
+#pragma unroll
+                    for (int j = 0; j < W; j++)
+                        w.e[j] = skip == 1 && j < 3 ? all[(j + 1) & 3] : skip == 2 && j < 2 ? all[(j + 2) & 3]
+                                 : skip == 3 && j < 1 ? all[3] : 0.0f;
+                }
+                if (Q % 64 == 0 || lane + 64 * i < Q) *(typename vec_t<float, W>::reg *)(bc + e) = w.e;
+            }
             // (one wave: what it writes to LDS is there for its next reads)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             if (t + U < hi) load(t + U);
             if (p.softplus) {
 #pragma unroll
-                for (int i = 0; i < U; i++) v[i] = scan_softplus(v[i]);
+                for (int i = 0; i < R; i++) v[i] = scan_softplus(v[i]);
             }
+#pragma unroll
+            for (int i = 0; i < R; i++) u[i] = v[i] * x[i];
             auto row = [&](int i) {
-                const float u = v[i] * x[i];
+                const float vi = scan_from<LPC>(v[i / P], i % P), ui = scan_from<LPC>(u[i / P], i % P);
                 const float *b = bc + i * K * RS + part * S, *c = b + RS;
                 float o[4];
 #pragma unroll
                 for (int n = 0; n < S; n++) {
-                    h[n] = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(v[i] * A[n]), u * b[n]);
+                    h[n] = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(vi * A[n]), ui * b[n]);
                     if (OUT) o[n & 3] = n < 4 ? h[n] * c[n] : __builtin_fmaf(h[n], c[n], o[n & 3]);
                 }
-                if (OUT) y[i] = scan_sum<LPC>((o[0] + o[1]) + (o[2] + o[3]));
-                else sum += v[i];
+                if (OUT) {
+                    const float all = scan_sum<LPC>((o[0] + o[1]) + (o[2] + o[3]));
+                    y[i / P] = i % P == 0 || own == i % P ? all : y[i / P];
+                }
             };
             auto out = [&](int n) {
 #pragma unroll
-                for (int i = 0; i < U; i++) y[i] = __builtin_fmaf(skip, x[i], y[i]);
+                for (int i = 0; i < R; i++) y[i] = __builtin_fmaf(skip, x[i], y[i]);
                 if (p.z) {
 #pragma unroll
-                    for (int i = 0; i < U; i++) y[i] *= rows_silu(z[i]);
+                    for (int i = 0; i < R; i++) y[i] *= rows_silu(z[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < U; i++)
-                    if (n == U || i < n)
-                        *(T *)((char *)((T *)p.y + (size_t)(t + i) * p.ldy) + at) = (T)y[i];
+                for (int i = 0; i < R; i++) {
+                    const int r = i * P + (P > 1 ? own : 0);
+                    if ((n == U || r < n) && (P == LPC || part < P))
+                        *(T *)((char *)((T *)p.y + (size_t)(t + r) * p.ldy) + at) = (T)y[i];
+                }
             };
+            if (!OUT) {
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    if (t + i * P + own < hi && part < P) sum += v[i];
+            }
             if (t + U <= hi) {
 #pragma unroll
                 for (int i = 0; i < U; i++) row(i);
                 if (OUT) out(U);
             } else {
 #pragma unroll
-                for (int i = 0; i < U; i++) {
-                    y[i] = 0.0f;
+                for (int i = 0; i < R; i++) y[i] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < U; i++)
                     if (t + i < hi) row(i);
-                }
                 if (OUT) out(hi - t);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
-        return sum;
+        return scan_sum<LPC>(sum);
     }
 };
 
@@ -373,33 +430,44 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
     }
 }
 
-// The split of a packed batch of prompts: chunk = 0, a wave (per 64 / lanes
-// channels) for each sequence, or chunks of so many rows, whose states are
-// computed twice. Both sides' times as a model that fits what was measured:
-// one bf16 prompt of 4,096 rows, 4,608 channels and 16 states takes 1,800 us
-// as a sequence per wave and 177 us in 40 chunks (72 + 9 + 96); 13 sequences
-// of 1,999 rows with 2,304 channels and 64 states, the longest of about 400,
-// take 180 us and 166; 60 of about 100 rows each are faster by themselves.
+// How a packed batch of prompts is split: S states of a channel to a lane,
+// and chunk = 0, a wave (per 64 / lanes channels) for each sequence, or chunks
+// of so many rows, whose states are computed twice.
+// A wave's rows come one after the other, so few long sequences want many
+// waves of few rows each, and a short batch wants few states to a lane; but
+// chunks cost their second computation and two more launches, and a lane of
+// 4 states more in all than one of 16. The choice is the least of a model, in
+// ns, of what was measured: a row of a wave by itself (`alone`), a row among
+// as many waves as keep the SIMDs busy (`rows`, and `part` for the chunks'
+// first pass), and what the launches take. One bf16 prompt of 4,608 channels
+// and 16 states: 4,096 rows take 1,840 us in one piece, 609 with 4 states a
+// lane, 180 in 40 chunks (75 + 9 + 96), 400 rows 176, 63 and 38; 1,999 f32
+// rows of 2,304 channels and 64 states in chunks 145 (57 + 8 + 80).
 struct scan_plan {
-    int lanes, chunk, chunks;
+    int S, lanes, chunk, chunks;
+    double ns;
 };
-static scan_plan scan_split(int tokens, int D, int N, int n_seq, int longest) {
-    scan_plan r = {1, 0, 0};
-    while (r.lanes * 16 < N) r.lanes *= 2;
-    // ns of a row: of a wave by itself (memory's latency), and of one among
-    // as many as keep the SIMDs busy
-    const double simds = 1024, waves = ((double)D * r.lanes + 63) / 64, states = N < 16 ? N : 16;
-    const double alone = 440, all = 14 * states + 112, part = 11 * states + 76;
-    const double rows = tokens * waves / simds;
-    if (longest <= 0 || longest > tokens) longest = tokens;
-    double most = 3 * simds / waves;              // three waves to a SIMD, as registers allow
+static scan_plan scan_try(int S, int lanes, int tokens, int D, int longest) {
+    const double simds = 1024, waves = ((double)D * lanes + 63) / 64, load = tokens * waves / simds;
+    const double alone = 70 + 21 * S + 60.0 / lanes, rows = 40 + 15 * S + 65.0 / lanes, part = 20 + 11 * S + 60.0 / lanes;
+    scan_plan r = {S, lanes, 0, 0, 6000 + fmax(alone * longest, rows * load)};
+    double most = (S == 16 ? 3 : S == 8 ? 4 : 5) * simds / waves;        // as many to a SIMD as registers allow
     if (most > tokens / 16) most = tokens / 16;
     if (most < 2) return r;
     const int chunk = ((int)(tokens / most) + 7) / 8 * 8, chunks = (tokens + chunk - 1) / chunk;
-    const double direct = fmax(alone * longest, all * rows);
-    const double split = fmax(alone * chunk, all * rows) + fmax(0.75 * alone * chunk, part * rows) + 15000;
-    if (chunks >= 2 && split < direct) r.chunk = chunk, r.chunks = chunks;
+    const double ns = 25000 + fmax(alone * chunk, rows * load) + fmax(0.75 * alone * chunk, part * load);
+    if (chunks >= 2 && ns < r.ns) r = {S, lanes, chunk, chunks, ns};
     return r;
+}
+static scan_plan scan_split(int tokens, int D, int N, int longest) {
+    if (longest <= 0 || longest > tokens) longest = tokens;
+    if (N <= 4) return scan_try(4, 1, tokens, D, longest);
+    int lanes = 2;
+    while (lanes * 4 < N) lanes *= 2;             // of 4 states each
+    if (N > 128) return scan_try(16, 16, tokens, D, longest);
+    const scan_plan few = N > 64 ? scan_try(8, 16, tokens, D, longest) : scan_try(4, lanes, tokens, D, longest);
+    const scan_plan many = N <= 8 ? scan_try(8, 1, tokens, D, longest) : scan_try(16, lanes / 4, tokens, D, longest);
+    return few.ns < many.ns ? few : many;
 }
 static size_t scan_floats(const scan_plan &s, int D, int N) {
     return s.chunk ? (size_t)s.chunks * (2 * (size_t)D * N + D + 1) : 0;
@@ -424,16 +492,24 @@ static void scan_token_launch(const scan_p &p, hipStream_t st) {
 }
 
 template <typename T>
-static void scan_launch(const scan_p &p, hipStream_t st) {
+static void scan_launch(const scan_p &p, const scan_plan &s, hipStream_t st) {
     const int N = p.N;
     if (p.starts) {
-        if (N <= 4) scan_rows_launch<T, 4, 1, 8>(p, st);
-        else if (N <= 8) scan_rows_launch<T, 8, 1, 8>(p, st);
-        else if (N <= 16) scan_rows_launch<T, 16, 1, 4>(p, st);
-        else if (N <= 32) scan_rows_launch<T, 16, 2, 4>(p, st);
-        else if (N <= 64) scan_rows_launch<T, 16, 4, 4>(p, st);
-        else if (N <= 128) scan_rows_launch<T, 16, 8, 4>(p, st);
-        else scan_rows_launch<T, 16, 16, 2>(p, st);
+#define SCAN(S_, L_, U_) \
+    if (s.S == S_ && s.lanes == L_) return scan_rows_launch<T, S_, L_, U_>(p, st)
+        SCAN(4, 1, 8);
+        SCAN(4, 2, 8);
+        SCAN(4, 4, 8);
+        SCAN(4, 8, 8);
+        SCAN(4, 16, 8);
+        SCAN(8, 1, 8);
+        SCAN(8, 16, 8);
+        SCAN(16, 1, 4);
+        SCAN(16, 2, 4);
+        SCAN(16, 4, 4);
+        SCAN(16, 8, 8);
+        SCAN(16, 16, 4);
+#undef SCAN
     } else {
         if (N < 4) scan_token_launch<T, 1, 4>(p, st);
         else if (N == 4) scan_token_launch<T, 4, 1>(p, st);
@@ -446,21 +522,21 @@ static void scan_launch(const scan_p &p, hipStream_t st) {
     }
 }
 
-extern "C" size_t wk_scan_work(int tokens, int D, int N, int n_seq, int longest) {
-    return scan_floats(scan_split(tokens, D, N, n_seq, longest), D, N) * 4;
+extern "C" size_t wk_scan_work(int tokens, int D, int N, int longest) {
+    return scan_floats(scan_split(tokens, D, N, longest), D, N) * 4;
 }
 
 extern "C" int wk_selective_scan(const warp_hip_scan_args *a, void *stream) {
     const size_t dn = (size_t)a->channels * a->states;
-    scan_plan s = {0, 0, 0};
-    if (a->starts) s = scan_split(a->tokens, a->channels, a->states, a->n_seq, a->longest);
+    scan_plan s = {0, 0, 0, 0, 0};
+    if (a->starts) s = scan_split(a->tokens, a->channels, a->states, a->longest);
     float *w = (float *)a->work;
     scan_p p = {a->tokens, a->n_seq, a->channels, a->states, a->groups, a->n_slots, a->softplus, s.chunk, s.chunks,
                 a->starts, a->slots, a->x, a->dt, a->B, a->C, a->z, a->ldx, a->lddt, a->ldbc, a->ldz, a->ldy,
                 a->A, a->D, a->dt_bias, a->state_in, a->state_out, a->y,
                 w, w + 2 * s.chunks * dn, w + s.chunks * dn, (int *)(w + s.chunks * (2 * dn + a->channels))};
-    if (a->type == WARP_HIP_F32) scan_launch<float>(p, (hipStream_t)stream);
-    else if (a->type == WARP_HIP_BF16) scan_launch<bf16_t>(p, (hipStream_t)stream);
-    else scan_launch<f16_t>(p, (hipStream_t)stream);
+    if (a->type == WARP_HIP_F32) scan_launch<float>(p, s, (hipStream_t)stream);
+    else if (a->type == WARP_HIP_BF16) scan_launch<bf16_t>(p, s, (hipStream_t)stream);
+    else scan_launch<f16_t>(p, s, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
