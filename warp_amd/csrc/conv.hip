@@ -7,9 +7,10 @@
 //
 // What bounds it is memory: each input is read once, each output written
 // once, about 19 issue slots of the vector units between them (four taps, and
-// SiLU's two instructions at a quarter of the rate), half of the time memory
-// takes. 8,191 bf16 rows of 4,640 channels in 11 sequences: 35.6 us, 4.3 TB/s
-// (a copy of that size reaches 4.7); 46 us with stores that go through L2.
+// SiLU's two instructions at half of the rate), half of the time memory takes.
+// 8,191 bf16 rows of 4,640 channels in 11 sequences: 30.4 us, 5.0 TB/s (a copy
+// that leaves the caches behind reaches 4.7); a quarter more with stores that
+// go through L2.
 
 #include "rows.h"
 #include "warp_internal.h"
@@ -28,15 +29,20 @@ struct conv_p {
 };
 
 // A thread's V channels: weights and bias in registers, taps aligned to the
-// end of the window (KS = 0: any number of taps up to CONV_MAX_TAPS).
+// end of the window (KS = 0: any number of taps up to CONV_MAX_TAPS, for rows
+// shorter than a vector). Up to three taps a vector is 16 bytes, above that 8:
+// weights and window grow with the taps, and four of 16 bytes leave three
+// waves to a SIMD (8,191 rows of 4,640 bf16 36.1 us, 31.5 with 8 bytes; with
+// any number of taps in a loop, three take 54.8 us, so 31.6).
 template <typename T, int KS, bool ONE>
 struct conv_t {
-    static constexpr int V = rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS;
+    static constexpr int V = KS > 3 ? rows_of<T>::V / 2 : rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS;
+    typedef cols_t<T, ONE, V> cols;
     float w[NT][V], b[V];
     int first;                                    // of the window's NT places that hold a tap
     bool silu;
 
-    __device__ __forceinline__ conv_t(const conv_p &p, const cols_t<T, ONE> &k) {
+    __device__ __forceinline__ conv_t(const conv_p &p, const cols &k) {
         first = KS ? 0 : NT - p.taps;
         silu = p.silu;
 #pragma unroll
@@ -72,10 +78,10 @@ struct conv_t {
 // One token of each of n_seq sequences: a thread takes V channels of one.
 template <typename T, int KS, bool ONE>
 __global__ __launch_bounds__(256) void k_conv_token(conv_p p) {
-    constexpr int V = rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS;
+    constexpr int V = conv_t<T, KS, ONE>::V, NT = conv_t<T, KS, ONE>::NT;
     const int c0 = ((int)blockIdx.x * (int)blockDim.x + (int)threadIdx.x) * V;
     if (c0 >= p.C) return;
-    const cols_t<T, ONE> k(c0, p.C);
+    const typename conv_t<T, KS, ONE>::cols k(c0, p.C);
     const conv_t<T, KS, ONE> conv(p, k);
     const int hist = NT - 1 - conv.first;
     for (int s = blockIdx.y; s < p.n_seq; s += gridDim.y) {
@@ -113,13 +119,13 @@ __global__ __launch_bounds__(256) void k_conv_token(conv_p p) {
 // may be state_in: what a thread uses of a slot's state nobody else writes.
 template <typename T, int KS, bool ONE>
 __global__ __launch_bounds__(256) void k_conv_rows(conv_p p) {
-    constexpr int V = rows_of<T>::V, NT = KS ? KS : CONV_MAX_TAPS, U = 4;
+    constexpr int V = conv_t<T, KS, ONE>::V, NT = conv_t<T, KS, ONE>::NT, U = 4;
     typedef vec_t<T, V> vec;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c0 = ((int)blockIdx.x * 64 + lane) * V, runs = max(1, (p.tokens + p.run - 1) / p.run);
     const seqs_t seqs(p.starts, p.slots, p.n_seq, p.tokens, p.n_slots);
     const bool live = c0 < p.C;
-    const cols_t<T, ONE> k(live ? c0 : p.C - 1, p.C);
+    const typename conv_t<T, KS, ONE>::cols k(live ? c0 : p.C - 1, p.C);
     const conv_t<T, KS, ONE> conv(p, k);
     const int hist = NT - 1 - conv.first;
     const T *x = (const T *)p.x + k.c;
@@ -177,27 +183,38 @@ __global__ __launch_bounds__(256) void k_conv_rows(conv_p p) {
 
 template <typename T, int KS, bool ONE>
 static void conv_launch(conv_p p, hipStream_t st) {
-    constexpr int V = rows_of<T>::V;
+    constexpr int V = conv_t<T, KS, ONE>::V;
     const int cols = ((p.C + V - 1) / V + 63) / 64;
     if (!p.starts) {
-        hipLaunchKernelGGL((k_conv_token<T, KS, ONE>), dim3(cols, p.n_seq < 32768 ? p.n_seq : 32768), dim3(64), 0, st, p);
+        // (waves that take sequences in turn load their weights once: 400
+        // sequences of 8,000 bf16 channels 13.7 us, 18.6 with a wave each)
+        const int most = 2048 / cols + 1;
+        hipLaunchKernelGGL((k_conv_token<T, KS, ONE>), dim3(cols, p.n_seq < most ? p.n_seq : most), dim3(64), 0, st, p);
         return;
     }
-    // Runs of 16 rows read 3 of 19 twice and load their weights once, but a
-    // batch has to make enough waves of them: 7,000 rows of 1,024 channels take
-    // 13.8, 13.2 and 15.6 us in runs of 16, 8 and 4, 1,000 rows of 513 take 18.2,
-    // 11.6 and 7.8, the 8,191 of 4,640 below 35.6, 39.2 and 55.3.
-    const int64_t work = (int64_t)p.tokens * cols;
-    p.run = work >= 16 * 768 ? 16 : work >= 8 * 768 ? 8 : 4;
+    // Runs of 12 rows read 3 of 15 twice and load their weights once, but a
+    // batch has to make enough waves of them: in runs of 4, 8, 12 and 24,
+    // 8,191 bf16 rows of 4,640 channels take 38.6, 30.6, 30.4 and 33.1 us, 1,537
+    // f32 rows of 4,096 10.0, 10.0, 9.8 and 11.0, 300 f16 rows of 4,640 8.0, 8.5,
+    // 9.2 and 11.7, 1,000 f32 rows of 1,000 6.5, 6.7, 7.2 and 9.5.
+    p.run = (int64_t)p.tokens * cols >= 24576 ? 12 : 4;
     const int blocks = (p.tokens + 4 * p.run - 1) / (4 * p.run);
     hipLaunchKernelGGL((k_conv_rows<T, KS, ONE>), dim3(cols, blocks < 1 ? 1 : blocks < 32768 ? blocks : 32768), dim3(256), 0,
                        st, p);
 }
 template <typename T>
 static void conv_type(const conv_p &p, hipStream_t st) {
-    if (p.C < rows_of<T>::V) conv_launch<T, 0, true>(p, st);
-    else if (p.taps == 4) conv_launch<T, 4, false>(p, st);
-    else conv_launch<T, 0, false>(p, st);
+    if (p.C < rows_of<T>::V) return conv_launch<T, 0, true>(p, st);
+    switch (p.taps) {
+    case 1: return conv_launch<T, 1, false>(p, st);
+    case 2: return conv_launch<T, 2, false>(p, st);
+    case 3: return conv_launch<T, 3, false>(p, st);
+    case 4: return conv_launch<T, 4, false>(p, st);
+    case 5: return conv_launch<T, 5, false>(p, st);
+    case 6: return conv_launch<T, 6, false>(p, st);
+    case 7: return conv_launch<T, 7, false>(p, st);
+    default: return conv_launch<T, 8, false>(p, st);
+    }
 }
 
 extern "C" int wk_short_conv(const warp_hip_conv_args *a, void *stream) {

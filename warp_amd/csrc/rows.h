@@ -48,9 +48,8 @@ struct rows_of<f16_t> {
 // last thread's begins early, at C - V, so that it loads a whole vector too,
 // and it stores only what no other thread has: its elements from `skip` on.
 // ONE: rows shorter than a vector, element by element.
-template <typename T, bool ONE>
+template <typename T, bool ONE, int V = rows_of<T>::V>
 struct cols_t {
-    static constexpr int V = rows_of<T>::V;
     typedef vec_t<T, V> vec;
     int c, skip, n;                               // its first column; see above; elements there are
 
