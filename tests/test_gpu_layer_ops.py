@@ -42,7 +42,8 @@ RAGGED = [0, 5, 1, 0, 37, 2, 16, 3, 0]
 LONG = [130, 1, 0, 700, 64, 3, 333]
 
 
-def run_conv(rng, t, C, taps, lengths, *, single=False, silu=True, bias=True, state="in", pad=0, lead=0, behind=0, ld=0):
+def run_conv(rng, t, C, taps, lengths, *, single=False, silu=True, bias=True, state="in", pad=0, lead=0, behind=0, ld=0,
+             poison=False):
     n = len(lengths)
     starts, T = (None, n) if single else layout(lengths, lead, behind)
     n_slots = n + 2
@@ -55,6 +56,8 @@ def run_conv(rng, t, C, taps, lengths, *, single=False, silu=True, bias=True, st
     live = np.where((slots >= 0) & (slots < n_slots), slots, -1)
     y, e, new = lr.conv(x, w, b, silu, lr.spans(starts, n, T), live, h if state != "none" else h * 0)
     before_y, before_h = lr.pack(normal(rng, (T, C), t), t), lr.pack(normal(rng, h.shape, t), t)
+    if poison:                                    # what is not computed is not read
+        x[np.isnan(y)], h[np.setdiff1d(np.arange(n_slots), live)] = NAN, NAN
     xb, xp = strided(x, t, ld or C, (ld - C) // 2 if ld else 0)
     yb, hin = dev(before_y), dev(lr.pack(h, t))
     hout = hin if state == "inplace" else dev(before_h)
@@ -93,7 +96,7 @@ def test_conv_no_tokens_carries_states():
 
 
 def run_scan(rng, t, Ch, N, lengths, *, G=1, single=False, gate=True, skip=True, softplus=True, bias=True, state="in", pad=0,
-             lead=0, behind=0, wide=0, longest=None, rates=None):
+             lead=0, behind=0, wide=0, longest=None, rates=None, poison=False):
     n = len(lengths)
     starts, T = (None, n) if single else layout(lengths, lead, behind)
     n_slots = n + 2
@@ -115,6 +118,11 @@ def run_scan(rng, t, Ch, N, lengths, *, G=1, single=False, gate=True, skip=True,
     y, ye, new, ne = lr.scan(x, dt, A, B, Cc, D, z, db, softplus, lr.spans(starts, n, T), live,
                              None if state == "none" else h, n_slots)
     before_y, before_h = lr.pack(normal(rng, (T, Ch), t), t), (rng.normal(size=h.shape)).astype(np.float32)
+    if poison:
+        rows = np.isnan(y).any(1)
+        x[rows], dt[rows], B[rows], Cc[rows], h[np.setdiff1d(np.arange(n_slots), live)] = NAN, NAN, NAN, NAN, NAN
+        if gate:
+            z[rows] = NAN
     ldx, ldbc = Ch + wide, G * N + wide
     xb, xp = strided(x, t, ldx, wide // 2)
     Bb, Bp = strided(B.reshape(T, -1), t, ldbc, wide // 2)
@@ -304,3 +312,83 @@ def test_combine_gradient_against_differences():
         w2 = w.copy()
         w2[t, k] += 1
         assert abs(loss(y, w2) - base - dw[t, k]) <= lim
+
+
+def test_more_rows_than_a_grid_takes_at_once():
+    """Blocks that take further rows, sequences, tokens and pairs in turn."""
+    rng = np.random.default_rng(8)
+    run_conv(rng, "f32", 5, 2, [1_000_000, 0, 3, 700_000], state="inplace", silu=False)
+    run_conv(rng, "f32", 5, 4, [1] * 9000, single=True, state="inplace", pad=3000)
+    run_scan(rng, "f32", 2, 4, [1] * 20000, single=True, state="inplace", pad=3000)
+    run_scan(rng, "f32", 2, 4, [1] * 33000 + [0] * 3000 + [2] * 500, state="inplace", pad=3000)
+
+
+@pytest.mark.parametrize("T,K,E,H", [(300000, 2, 7, 4), (20, 70, 90, 33), (40, 130, 900, 9)])
+def test_dispatch_and_combine_of_many_pairs(T, K, E, H):
+    rng = np.random.default_rng(T + K)
+    idx = rng.integers(-1, E, size=(T, K)).astype(np.int32)
+    run_dispatch(idx, E, H, "bf16")
+    pos, y, w, r, d = places(rng, T, K, 0.1), normal(rng, (T * K, H), "f16"), rng.normal(size=(T, K)).astype(np.float32), normal(
+        rng, (T, H), "f16"), normal(rng, (T, H), "f16")
+    ref, err = lr.combine(y, pos, w, r)
+    out, pb, wb, yb = empty((T, H), np.float16), dev(pos), dev(w), dev(lr.pack(y, "f16"))
+    kw = dict(dtype=lr.TYPE["f16"], tokens=T, top_k=K, hidden=H, w=wb)
+    hip().expert_combine(yb, pb, out, resid=dev(lr.pack(r, "f16")), **kw)
+    lr.check(host(out), ref, err, "f16")
+    dy, dw, err = lr.combine_backward(d, y, pos, w)
+    before = np.ones((T * K, H), np.float16)
+    gb, gw = dev(before), empty((T, K))
+    hip().expert_combine_backward(dev(lr.pack(d, "f16")), yb, pb, gb, gw, **kw)
+    lr.check(host(gb), dy, np.abs(np.nan_to_num(dy)) * lr.EPS, "f16", before)
+    lr.check(host(gw), dw, err, "f32")
+
+
+def test_rows_that_are_not_computed_may_hold_anything():
+    """NaN in padding rows, in rows outside every sequence and in states of no sequence."""
+    rng = np.random.default_rng(12)
+    for lengths in (RAGGED, LONG):
+        run_conv(rng, "bf16", 70, 4, lengths, state="inplace", pad=3, lead=5, behind=4, poison=True)
+        run_scan(rng, "bf16", 70, 16, lengths, state="inplace", pad=3, lead=5, behind=4, poison=True, longest=0)
+        run_scan(rng, "f32", 33, 5, lengths, state="in", pad=3, lead=5, behind=4, poison=True)
+    run_conv(rng, "f32", 70, 4, [1] * 12, single=True, state="inplace", pad=5, poison=True)
+    run_scan(rng, "f32", 70, 16, [1] * 12, single=True, state="inplace", pad=5, poison=True)
+
+
+@pytest.mark.parametrize("N", [5, 16])
+@pytest.mark.parametrize("single", [False, True])
+def test_an_infinity_stays_in_its_channel_and_sequence(N, single):
+    """One infinite input, then one that is no number: every output and state of other channels, of other
+    sequences and of the rows before it is bit for bit what it is without."""
+    rng = np.random.default_rng(N)
+    wh, Ch, lengths = hip(), 37, [1] * 6 if single else [30, 0, 400, 21]
+    starts, T = (None, 6) if single else layout(lengths)
+    n = len(lengths)
+    x, dt, z = (normal(rng, (T, Ch), "f32", s) for s in (1, 0.3, 1))
+    BC, w = [normal(rng, (T, N), "f32") for _ in range(2)], rng.normal(size=(Ch, 4)).astype(np.float32)
+    A = -rng.uniform(0.1, 3, size=(Ch, N)).astype(np.float32)
+    st = dev(starts) if starts is not None else None
+    at, seq, c = (2, 2, 11) if single else (100, 2, 11)
+
+    def run(v):
+        x2 = x.copy()
+        x2[at, c] = v
+        rows = dict(dtype=0, tokens=T, channels=Ch, n_seq=n, n_slots=n, starts=st)
+        u, y, hist, h = empty((T, Ch)), empty((T, Ch)), empty((n, 3, Ch)), empty((n, Ch, N))
+        xb = dev(x2)
+        wh.short_conv(xb, dev(w), u, taps=4, state_out=hist, **rows)
+        need = 0 if single else wh.selective_scan_work(T, Ch, N, n)
+        wh.selective_scan(xb, dev(dt), dev(A), dev(BC[0]), dev(BC[1]), y, n_state=N, z=dev(z), state_out=h,
+                          work=empty(max(need, 16), np.uint8), work_bytes=need, **rows)
+        return host(u), host(y), host(hist), host(h)
+    want = run(x[at, c])
+    end = at + 1 if single else int(starts[seq + 1])
+    for v in (np.inf, -np.inf, NAN):
+        for k, (got, ref) in enumerate(zip(run(v), want)):
+            same = got.view(np.uint32) == ref.view(np.uint32)
+            touched = np.zeros(same.shape, bool)
+            if k < 2:
+                touched[at:end, c] = True
+            else:
+                touched[(seq, slice(None), c) if k == 2 else (seq, c)] = True
+            assert (same | touched).all()
+            assert k == 0 or k == 2 or not np.isfinite(got[at, c] if k == 1 else got[seq, c]).any()

@@ -128,3 +128,12 @@ def test_python_calls_raise():
     with pytest.raises(wh.WarpHipError) as e:
         wh.short_conv(A, A, A, dtype=wh.F32, tokens=1, channels=8, taps=4, n_seq=1, n_slots=1)
     assert e.value.code == wh.E_ARG
+
+
+def test_kernels_keep_to_registers(tmp_path):
+    from test_kernel_scratch import READELF, scratch_bytes
+    if READELF is None:
+        pytest.skip("llvm-readelf not installed")
+    got = {k: v for k, v in scratch_bytes(tmp_path).items() if any(n in k for n in ("k_conv_", "k_scan_", "k_sort_", "k_combine"))}
+    # (k_combine_lut and k_combine_chunk are the layer's own combines)
+    assert len(got) > 60 and max(v for k, v in got.items() if "lut" not in k and "chunk" not in k) == 0, got
