@@ -72,8 +72,8 @@ def test_scan_refuses_a_short_workspace():
                                     dict(offsets=None), dict(perm=None), dict(pos=None), dict(idx=A + 1), dict(offsets=A + 2),
                                     dict(perm=A + 3), dict(pos=A + 2), dict(x=None), dict(xs=None), dict(type=5),
                                     dict(hidden=0), dict(hidden=(1 << 24) + 1), dict(ldx=15), dict(ldxs=15), dict(x=A + 2),
-                                    dict(xs=A + 1), dict(tokens=2000, work=None), dict(tokens=2000, work=A + 2),
-                                    dict(tokens=2000, work_bytes=4), dict(tokens=(1 << 29) + 1),
+                                    dict(xs=A + 1), dict(tokens=5000, work=None), dict(tokens=5000, work=A + 2),
+                                    dict(tokens=5000, work_bytes=4), dict(tokens=(1 << 29) + 1),
                                     dict(tokens=1 << 30, top_k=2)])
 def test_dispatch_refuses(change):
     assert refused(wh.lib().warp_hip_expert_dispatch, dispatch(), **change) == wh.E_ARG

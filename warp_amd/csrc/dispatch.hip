@@ -213,8 +213,9 @@ __global__ __launch_bounds__(256) void k_sort_rows(sort_p p, int parts) {
 // All of it at once where a block can sort all pairs: every block does, into
 // LDS, and copies its share of the rows (the first also writes the lists).
 // Three launches take 15 us for 32 tokens of 7,168 bf16 to 16 of 384 experts,
-// this one 6.9.
-constexpr int SMALL_PAIRS = 2048;
+// this one 6.9; 500 tokens of 1,012 to 8 of 239 11.2, 520 in three launches 14.4
+// and the gaps between them.
+constexpr int SMALL_PAIRS = 4096;
 template <typename T, bool ONE, int STEPS>
 __global__ __launch_bounds__(64 * SORT_WAVES) void k_sort_small(sort_p p, int parts) {
     extern __shared__ int lds[];                  // [pairs] places, [E] beginnings, [SORT_WAVES][E] counts
@@ -274,10 +275,10 @@ static void dispatch_launch(sort_p p, hipStream_t st) {
         const int parts = (vecs + 63) / 64, blocks = p.xs ? (p.tokens * parts + SORT_WAVES - 1) / SORT_WAVES : 1;
         const dim3 grid(blocks < 1 ? 1 : blocks < 256 ? blocks : 256);
         const size_t lds = (p.pairs + p.E) * sizeof(int) + SORT_WAVES * p.E * sizeof(uint16_t);
-        if (p.pairs <= 64 * SORT_WAVES)
-            hipLaunchKernelGGL((k_sort_small<T, ONE, 1>), grid, dim3(64 * SORT_WAVES), lds, st, p, parts);
-        else hipLaunchKernelGGL((k_sort_small<T, ONE, SMALL_PAIRS / SORT_WAVES / 64>), grid, dim3(64 * SORT_WAVES), lds, st, p,
-                                parts);
+        constexpr int step = 64 * SORT_WAVES;
+        if (p.pairs <= step) hipLaunchKernelGGL((k_sort_small<T, ONE, 1>), grid, dim3(step), lds, st, p, parts);
+        else if (p.pairs <= 4 * step) hipLaunchKernelGGL((k_sort_small<T, ONE, 4>), grid, dim3(step), lds, st, p, parts);
+        else hipLaunchKernelGGL((k_sort_small<T, ONE, SMALL_PAIRS / step>), grid, dim3(step), lds, st, p, parts);
         return;
     }
     const size_t lds = SORT_WAVES * p.E * sizeof(uint16_t);
@@ -371,37 +372,58 @@ __global__ __launch_bounds__(256) void k_combine(comb_p p, int parts) {
     }
 }
 
-// A wave takes one pair: its row of dy, and the product of its row of y with
-// the token's dout (which the token's other pairs find in the caches). 8,192
-// tokens of 2,304 bf16, 8 rows each: 118 us, 5.4 TB/s.
-template <typename T, bool ONE>
+// W waves take a pair: its row of dy, and the product of its row of y with
+// the token's dout (which the token's other pairs find in the caches). Many
+// short waves beat fewer that hold more: with two or four pairs to a wave the
+// 117 us below are 133 and 137. 8,192 tokens of 2,304 bf16, 8 rows each: 117
+// us, 5.5 TB/s. Few pairs get four waves each: 10 tokens of 2,304 f32, 8 rows
+// each, take 8.4 us with one and 4.1 with four; 8,192 as above 118 and 153.
+template <typename T, bool ONE, int W>
 __global__ __launch_bounds__(256) void k_combine_back(comb_p p) {
-    constexpr int V = rows_of<T>::V;
+    constexpr int V = rows_of<T>::V, CU = 4;               // vectors a lane loads at once
+    __shared__ float part[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int pairs = p.tokens * p.K;
-    for (int i = (int)blockIdx.x * 4 + wave; i < pairs; i += (int)gridDim.x * 4) {
+    const int pairs = p.tokens * p.K, own = wave % W;
+    for (int64_t i = (int64_t)blockIdx.x * (4 / W) + wave / W; i < pairs; i += (int64_t)gridDim.x * (4 / W)) {
         const int at = p.pos[i];
         float sum = 0.0f;
         if ((unsigned)at < (unsigned)pairs) {
             const float w = p.w ? p.w[i] : 1.0f;
-            const T *d = (const T *)p.dout + (size_t)(i / p.K) * p.ldd, *y = (const T *)p.y + (size_t)at * p.ldy;
+            const T *d = (const T *)p.dout + (size_t)((int)i / p.K) * p.ldd, *y = (const T *)p.y + (size_t)at * p.ldy;
             T *dy = (T *)p.dy + (size_t)at * p.lddy;
-            for (int c0 = lane * V; c0 < p.hidden; c0 += 64 * V) {
-                const cols_t<T, ONE> c(c0, p.hidden);
-                const vec_t<T, V> dv = c.load(d + c.c);
-                vec_t<T, V> yv, o;
-                yv.e = 0;
-                if (p.dw) yv = c.take(y + c.c);
+            for (int c0 = (own * 64 + lane) * V; c0 < p.hidden; c0 += CU * W * 64 * V) {
+                vec_t<T, V> dv[CU], yv[CU];
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    if (e >= c.skip) sum = __builtin_fmaf((float)dv.e[e], (float)yv.e[e], sum);
-                    o.e[e] = (T)(w * (float)dv.e[e]);
-                }
-                if (p.dy) c.stream(dy + c.c, o);
+                for (int u = 0; u < CU; u++)
+                    if (c0 + u * W * 64 * V < p.hidden) {
+                        const cols_t<T, ONE> c(c0 + u * W * 64 * V, p.hidden);
+                        dv[u] = c.load(d + c.c);
+                        if (p.dw) yv[u] = c.take(y + c.c);
+                    }
+#pragma unroll
+                for (int u = 0; u < CU; u++)
+                    if (c0 + u * W * 64 * V < p.hidden) {
+                        const cols_t<T, ONE> c(c0 + u * W * 64 * V, p.hidden);
+                        vec_t<T, V> o;
+#pragma unroll
+                        for (int e = 0; e < V; e++) {
+                            if (p.dw && e >= c.skip) sum = __builtin_fmaf((float)dv[u].e[e], (float)yv[u].e[e], sum);
+                            o.e[e] = (T)(w * (float)dv[u].e[e]);
+                        }
+                        if (p.dy) c.stream(dy + c.c, o);
+                    }
             }
         }
+        if (!p.dw) continue;
+#pragma unroll
         for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m);
-        if (p.dw && lane == 0) p.dw[i] = sum;
+        if (W > 1) {
+            if (lane == 0) part[wave] = sum;
+            __syncthreads();
+            sum = (part[0] + part[1]) + (part[2] + part[3]);
+            __syncthreads();
+        }
+        if (lane == 0 && own == 0) p.dw[i] = sum;
     }
 }
 
@@ -414,12 +436,20 @@ static void combine_launch(const comb_p &p, hipStream_t st) {
     if (p.hidden < V) hipLaunchKernelGGL((k_combine<T, true>), grid, dim3(256), 0, st, p, parts);
     else hipLaunchKernelGGL((k_combine<T, false>), grid, dim3(256), 0, st, p, parts);
 }
-template <typename T>
+template <typename T, bool ONE>
 static void combine_back_launch(const comb_p &p, hipStream_t st) {
-    const int64_t blocks = ((int64_t)p.tokens * p.K + 3) / 4;
+    // (four waves where one to each pair leaves SIMDs without any)
+    const int64_t pairs = (int64_t)p.tokens * p.K;
+    const int W = pairs < 4096 && p.hidden > 64 * rows_of<T>::V ? 4 : 1;
+    const int64_t blocks = (pairs * W + 3) / 4;
     const dim3 grid(blocks < 65536 ? blocks : 65536);
-    if (p.hidden < rows_of<T>::V) hipLaunchKernelGGL((k_combine_back<T, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((k_combine_back<T, false>), grid, dim3(256), 0, st, p);
+    if (W == 4) hipLaunchKernelGGL((k_combine_back<T, ONE, 4>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((k_combine_back<T, ONE, 1>), grid, dim3(256), 0, st, p);
+}
+template <typename T>
+static void combine_back_type(const comb_p &p, hipStream_t st) {
+    if (p.hidden < rows_of<T>::V) combine_back_launch<T, true>(p, st);
+    else combine_back_launch<T, false>(p, st);
 }
 
 extern "C" int wk_expert_combine(const warp_hip_combine_args *a, void *stream) {
@@ -434,8 +464,8 @@ extern "C" int wk_expert_combine(const warp_hip_combine_args *a, void *stream) {
 extern "C" int wk_expert_combine_backward(const warp_hip_combine_back_args *a, void *stream) {
     const comb_p p = {a->tokens, a->top_k, a->hidden, a->y, a->pos, a->w, nullptr, nullptr, a->dout, a->dy, a->dw,
                       a->ldy, 0, 0, a->ldd, a->lddy};
-    if (a->type == WARP_HIP_F32) combine_back_launch<float>(p, (hipStream_t)stream);
-    else if (a->type == WARP_HIP_BF16) combine_back_launch<bf16_t>(p, (hipStream_t)stream);
-    else combine_back_launch<f16_t>(p, (hipStream_t)stream);
+    if (a->type == WARP_HIP_F32) combine_back_type<float>(p, (hipStream_t)stream);
+    else if (a->type == WARP_HIP_BF16) combine_back_type<bf16_t>(p, (hipStream_t)stream);
+    else combine_back_type<f16_t>(p, (hipStream_t)stream);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
