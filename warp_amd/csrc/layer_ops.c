@@ -85,7 +85,7 @@ int warp_hip_short_conv(const warp_hip_conv_args *args, void *stream)
 size_t warp_hip_selective_scan_work(int tokens, int channels, int states, int n_seq, int longest)
 {
     if (tokens < 1 || channels < 1 || states < 1 || states > SCAN_MAX_STATES || n_seq < 1) return 0;
-    return wk_scan_work(tokens, channels, states, longest);
+    return wk_scan_work(tokens, channels, states, n_seq, longest);
 }
 
 int warp_hip_selective_scan(const warp_hip_scan_args *args, void *stream)
@@ -109,7 +109,7 @@ int warp_hip_selective_scan(const warp_hip_scan_args *args, void *stream)
     if (a.tokens && (!a.x || !a.dt || !a.B || !a.C || !a.y)) return WARP_HIP_E_ARG;
     if (a.n_seq == 0) return 0;
     if (a.starts && a.tokens) {
-        const size_t need = wk_scan_work(a.tokens, a.channels, a.states, a.longest);
+        const size_t need = wk_scan_work(a.tokens, a.channels, a.states, a.n_seq, a.longest);
         if (need && (!a.work || a.work_bytes < need || off(a.work, 16))) return WARP_HIP_E_ARG;
     }
     QUEUE(wk_selective_scan(&a, stream));

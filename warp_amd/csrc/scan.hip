@@ -33,17 +33,15 @@ struct scan_p {
 constexpr float LOG2E = 1.44269504088896341f;
 
 // log(1 + e^v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, and log(1 + e) =
-// 2 atanh(s) with s = e / (2 + e) <= 1/3: the series to s^13 (the next term is
-// below 2^-27 of the sum). Small results keep their digits, as the time steps
-// of slow channels need them.
+// 2 atanh(s) with s = e / (2 + e) <= 1/3, whose series in s^2 over s is here
+// the polynomial of degree 4 with the least relative error on [0, 1/9], 4e-9.
+// Small results keep their digits, as the time steps of slow channels need them.
 __device__ __forceinline__ float scan_softplus(float v) {
     const float e = rows_exp(-__builtin_fabsf(v)), s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
-    float r = 1.0f / 13;
-    r = __builtin_fmaf(r, q, 1.0f / 11);
-    r = __builtin_fmaf(r, q, 1.0f / 9);
-    r = __builtin_fmaf(r, q, 1.0f / 7);
-    r = __builtin_fmaf(r, q, 1.0f / 5);
-    r = __builtin_fmaf(r, q, 1.0f / 3);
+    float r = 0.14089166f;
+    r = __builtin_fmaf(r, q, 0.13980304f);
+    r = __builtin_fmaf(r, q, 0.20012455f);
+    r = __builtin_fmaf(r, q, 0.33333158f);
     return __builtin_fmaf(2.0f * s, __builtin_fmaf(r, q, 1.0f), __builtin_fmaxf(v, 0.0f));
 }
 
@@ -435,38 +433,41 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
 // of so many rows, whose states are computed twice.
 // A wave's rows come one after the other, so few long sequences want many
 // waves of few rows each, and a short batch wants few states to a lane; but
-// chunks cost their second computation and two more launches, and a lane of
-// 4 states more in all than one of 16. The choice is the least of a model, in
+// chunks cost their second computation and two more launches, and lanes of 4
+// states more in all than lanes of 16. The choice is the least of a model, in
 // ns, of what was measured: a row of a wave by itself (`alone`), a row among
 // as many waves as keep the SIMDs busy (`rows`, and `part` for the chunks'
 // first pass), and what the launches take. One bf16 prompt of 4,608 channels
 // and 16 states: 4,096 rows take 1,840 us in one piece, 609 with 4 states a
-// lane, 180 in 40 chunks (75 + 9 + 96), 400 rows 176, 63 and 38; 1,999 f32
-// rows of 2,304 channels and 64 states in chunks 145 (57 + 8 + 80).
+// lane, 180 in 40 chunks (74 + 9 + 98), 400 rows 176, 63 and 38. 1,999 f32 rows
+// of 2,304 channels and 64 states in 13 sequences: 145 in chunks (57 + 8 + 80)
+// or, as their lengths are more or less even, 120 to 187 a wave to a sequence.
 struct scan_plan {
     int S, lanes, chunk, chunks;
     double ns;
 };
-static scan_plan scan_try(int S, int lanes, int tokens, int D, int longest) {
+static scan_plan scan_try(int S, int lanes, int tokens, int D, int n_seq, int longest) {
     const double simds = 1024, waves = ((double)D * lanes + 63) / 64, load = tokens * waves / simds;
     const double alone = 70 + 21 * S + 60.0 / lanes, rows = 40 + 15 * S + 65.0 / lanes, part = 20 + 11 * S + 60.0 / lanes;
-    scan_plan r = {S, lanes, 0, 0, 6000 + fmax(alone * longest, rows * load)};
+    // (a sequence longer than the others runs on by itself)
+    const double over = longest - (double)tokens / n_seq;
+    scan_plan r = {S, lanes, 0, 0, fmax(5000 + alone * longest, rows * load + alone * fmax(over, 0))};
     double most = (S == 16 ? 3 : S == 8 ? 4 : 5) * simds / waves;        // as many to a SIMD as registers allow
     if (most > tokens / 16) most = tokens / 16;
     if (most < 2) return r;
     const int chunk = ((int)(tokens / most) + 7) / 8 * 8, chunks = (tokens + chunk - 1) / chunk;
-    const double ns = 25000 + fmax(alone * chunk, rows * load) + fmax(0.75 * alone * chunk, part * load);
+    const double ns = 8000 + fmax(8000 + alone * chunk, rows * load) + fmax(8000 + 0.75 * alone * chunk, part * load);
     if (chunks >= 2 && ns < r.ns) r = {S, lanes, chunk, chunks, ns};
     return r;
 }
-static scan_plan scan_split(int tokens, int D, int N, int longest) {
+static scan_plan scan_split(int tokens, int D, int N, int n_seq, int longest) {
     if (longest <= 0 || longest > tokens) longest = tokens;
-    if (N <= 4) return scan_try(4, 1, tokens, D, longest);
+    auto best = [&](int S, int lanes) { return scan_try(S, lanes, tokens, D, n_seq, longest); };
+    if (N <= 4) return best(4, 1);
+    if (N > 128) return best(16, 16);
     int lanes = 2;
     while (lanes * 4 < N) lanes *= 2;             // of 4 states each
-    if (N > 128) return scan_try(16, 16, tokens, D, longest);
-    const scan_plan few = N > 64 ? scan_try(8, 16, tokens, D, longest) : scan_try(4, lanes, tokens, D, longest);
-    const scan_plan many = N <= 8 ? scan_try(8, 1, tokens, D, longest) : scan_try(16, lanes / 4, tokens, D, longest);
+    const scan_plan few = N > 64 ? best(8, 16) : best(4, lanes), many = N <= 8 ? best(8, 1) : best(16, lanes / 4);
     return few.ns < many.ns ? few : many;
 }
 static size_t scan_floats(const scan_plan &s, int D, int N) {
@@ -522,14 +523,14 @@ static void scan_launch(const scan_p &p, const scan_plan &s, hipStream_t st) {
     }
 }
 
-extern "C" size_t wk_scan_work(int tokens, int D, int N, int longest) {
-    return scan_floats(scan_split(tokens, D, N, longest), D, N) * 4;
+extern "C" size_t wk_scan_work(int tokens, int D, int N, int n_seq, int longest) {
+    return scan_floats(scan_split(tokens, D, N, n_seq, longest), D, N) * 4;
 }
 
 extern "C" int wk_selective_scan(const warp_hip_scan_args *a, void *stream) {
     const size_t dn = (size_t)a->channels * a->states;
     scan_plan s = {0, 0, 0, 0, 0};
-    if (a->starts) s = scan_split(a->tokens, a->channels, a->states, a->longest);
+    if (a->starts) s = scan_split(a->tokens, a->channels, a->states, a->n_seq, a->longest);
     float *w = (float *)a->work;
     scan_p p = {a->tokens, a->n_seq, a->channels, a->states, a->groups, a->n_slots, a->softplus, s.chunk, s.chunks,
                 a->starts, a->slots, a->x, a->dt, a->B, a->C, a->z, a->ldx, a->lddt, a->ldbc, a->ldz, a->ldy,

@@ -420,7 +420,7 @@ int wk_kda(int T, int H, int K, int V, const float *q, const float *k, const flo
  * arguments checked and their strides filled in. 0, or not. */
 int wk_short_conv(const warp_hip_conv_args *a, void *stream);
 int wk_selective_scan(const warp_hip_scan_args *a, void *stream);
-size_t wk_scan_work(int tokens, int channels, int states, int longest);
+size_t wk_scan_work(int tokens, int channels, int states, int n_seq, int longest);
 int wk_expert_dispatch(const warp_hip_dispatch_args *a, void *stream);
 size_t wk_dispatch_work(int tokens, int top_k, int n_experts);
 int wk_expert_combine(const warp_hip_combine_args *a, void *stream);
