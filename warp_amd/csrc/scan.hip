@@ -260,12 +260,19 @@ struct scan_t {
             for (int i = 0; i < R; i++) u[i] = v[i] * x[i];
             auto row = [&](int i) {
                 const float vi = scan_from<LPC>(v[i / P], i % P), ui = scan_from<LPC>(u[i / P], i % P);
-                const float *b = bc + i * K * RS + part * S, *c = b + RS;
-                float o[4];
+                // (in fours of their own accord: as single loads some went out in twos)
+                typedef vec_t<float, 4>::reg four;
+                const four *b = (const four *)(bc + i * K * RS + part * S), *c = b + RS / 4;
+                four o = 0;
 #pragma unroll
-                for (int n = 0; n < S; n++) {
-                    h[n] = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(vi * A[n]), ui * b[n]);
-                    if (OUT) o[n & 3] = n < 4 ? h[n] * c[n] : __builtin_fmaf(h[n], c[n], o[n & 3]);
+                for (int m = 0; m < S / 4; m++) {
+                    const four bm = b[m], cm = OUT ? c[m] : bm;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int n = 4 * m + j;
+                        h[n] = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(vi * A[n]), ui * bm[j]);
+                        if (OUT) o[j] = m == 0 ? h[n] * cm[j] : __builtin_fmaf(h[n], cm[j], o[j]);
+                    }
                 }
                 if (OUT) {
                     const float all = scan_sum<LPC>((o[0] + o[1]) + (o[2] + o[3]));
