@@ -446,7 +446,7 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
 // as many waves as keep the SIMDs busy (`rows`, and `part` for the chunks'
 // first pass), and what the launches take. One bf16 prompt of 4,608 channels
 // and 16 states: 4,096 rows take 1,840 us in one piece, 609 with 4 states a
-// lane, 180 in 40 chunks (74 + 9 + 98), 400 rows 176, 63 and 38. 1,999 f32 rows
+// lane, 173 in 41 chunks (70 + 9 + 94), 400 rows 176, 63 and 38. 1,999 f32 rows
 // of 2,304 channels and 64 states in 13 sequences: 145 in chunks (57 + 8 + 80)
 // or, as their lengths are more or less even, 120 to 187 a wave to a sequence.
 struct scan_plan {
@@ -462,7 +462,8 @@ static scan_plan scan_try(int S, int lanes, int tokens, int D, int n_seq, int lo
     double most = (S == 16 ? 3 : S == 8 ? 4 : 5) * simds / waves;        // as many to a SIMD as registers allow
     if (most > tokens / 16) most = tokens / 16;
     if (most < 2) return r;
-    const int chunk = ((int)(tokens / most) + 7) / 8 * 8, chunks = (tokens + chunk - 1) / chunk;
+    // (a chunk more than fits would run by itself at the end)
+    const int chunk = ((tokens + (int)most - 1) / (int)most + 3) / 4 * 4, chunks = (tokens + chunk - 1) / chunk;
     const double ns = 8000 + fmax(8000 + alone * chunk, rows * load) + fmax(8000 + 0.75 * alone * chunk, part * load);
     if (chunks >= 2 && ns < r.ns) r = {S, lanes, chunk, chunks, ns};
     return r;
