@@ -142,9 +142,9 @@ __global__ __launch_bounds__(1024) void k_sort_scan(sort_p p) {
     if (threadIdx.x == 0) p.offsets[p.E] = base;
 }
 
-// 4,096 tokens of 2,304 bf16 to 8 of 256 experts: 33 us for the rows, 5.2 TB/s,
-// behind 9 for ranks and scan; with a block to 256 vectors of a row, the
-// places read pair by pair and stores through L2 48.6.
+// 4,096 tokens of 2,304 bf16 to 8 of 256 experts: 31 us for the rows, 5.4 TB/s,
+// behind 9 for ranks and scan (with four vectors a lane 32.4); with a block to
+// 256 vectors of a row, the places read pair by pair and stores through L2 48.6.
 // A part of a token's row, IT vectors a lane of a wave, and its copies to the
 // places of the token's pairs: at(i) is the place of pair i, a lane's each.
 template <typename T, bool ONE, int IT>
@@ -285,9 +285,9 @@ static void dispatch_launch(sort_p p, hipStream_t st) {
     if (p.per == 1024) hipLaunchKernelGGL((k_sort_rank<2>), dim3(p.blocks), dim3(64 * SORT_WAVES), lds, st, p);
     else hipLaunchKernelGGL((k_sort_rank<8>), dim3(p.blocks), dim3(64 * SORT_WAVES), lds, st, p);
     hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, p);
-    const int parts = p.xs ? (vecs + 255) / 256 : 1;
+    const int parts = p.xs ? (vecs + 127) / 128 : 1;
     const int64_t blocks = ((int64_t)p.tokens * parts + 3) / 4;
-    hipLaunchKernelGGL((k_sort_rows<T, ONE, 4>), dim3(blocks < 65536 ? blocks : 65536), dim3(256), 0, st, p, parts);
+    hipLaunchKernelGGL((k_sort_rows<T, ONE, 2>), dim3(blocks < 65536 ? blocks : 65536), dim3(256), 0, st, p, parts);
 }
 
 extern "C" int wk_expert_dispatch(const warp_hip_dispatch_args *a, void *stream) {
