@@ -176,6 +176,37 @@ def test_scan_rates_and_steps_at_their_ends():
     run_scan(rng, "f32", 64, 16, [1] * 9, single=True, rates=rates, state="inplace")
 
 
+@pytest.mark.parametrize("T", [160, 640])
+def test_scan_states_that_grow(T):
+    """Without a softplus a state may grow: by up to e^96 in the rows 16 .. 31, more than f32 can say, and back in the next
+    16. A state of zero stays zero meanwhile, and a small one is what it is row by row, however the rows are split."""
+    Ch, N, wh = 64, 16, hip()
+    rng = np.random.default_rng(T)
+    x, B, Cc = normal(rng, (T, Ch), "f32"), normal(rng, (T, 1, N), "f32"), normal(rng, (T, 1, N), "f32")
+    x[:64] = 0
+    dt = lr.rounded(rng.uniform(0.001, 0.01, size=(T, Ch)), "f32")
+    dt[16:32], dt[32:48] = 6, -6
+    A = rng.uniform(0.9, 1, size=(Ch, N)).astype(np.float32)
+    A[:, 0] = 1
+    h = np.zeros((1, Ch, N), np.float32)
+    h[0, Ch // 2:] = 1e-30
+    ref = lambda b, h: lr.scan(x[b:], dt[b:], A, B[b:], Cc[b:], None, None, None, False, [(0, T - b)], [0], h, 1)
+    y, ye, new, ne = ref(0, h)
+    # (of a zero state nothing is lost below f32's least number: the same from row 64 on)
+    zero = ref(64, None)
+    y[64:, :Ch // 2], ye[64:, :Ch // 2] = zero[0][:, :Ch // 2], zero[1][:, :Ch // 2]
+    new[:, :Ch // 2], ne[:, :Ch // 2] = zero[2][:, :Ch // 2], zero[3][:, :Ch // 2]
+    ye[:64, :Ch // 2] = 0
+    need = wh.selective_scan_work(T, Ch, N, 1, T)
+    assert need > 0 and np.isfinite(y).all()
+    yb, hb = dev(np.full((T, Ch), NAN, np.float32)), dev(h)
+    wh.selective_scan(dev(x), dev(dt), dev(A), dev(B), dev(Cc), yb, dtype=lr.TYPE["f32"], tokens=T, channels=Ch, n_state=N,
+                      n_seq=1, n_slots=1, starts=dev(np.array([0, T], np.int32)), state_in=hb, state_out=hb, softplus=False,
+                      longest=T, work=dev(np.full(need // 4, NAN, np.float32)), work_bytes=need)
+    lr.check(host(yb), y, ye, "f32")
+    lr.check(host(hb), new, ne, "f32")
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("Ch,N,G,n", [(1, 1, 1, 1), (4608, 16, 1, 3), (130, 16, 2, 70), (33, 4, 1, 5), (20, 8, 2, 3), (30, 24, 1, 4),
                                       (12, 64, 3, 2), (9, 128, 1, 3), (5, 256, 1, 2), (21, 5, 7, 9), (14, 23, 2, 3), (6, 33, 1, 2),

@@ -120,6 +120,7 @@ def test_accepted_arguments_reach_the_device():
 def test_workspace_sizes():
     assert wh.selective_scan_work(0, 64, 16, 1) == 0 and wh.selective_scan_work(64, 64, 257, 1) == 0
     assert wh.selective_scan_work(4096, 64, 16, 4096, 1) == 0          # a wave per sequence is enough
+    assert wh.selective_scan_work((1 << 30) + 1, 64, 16, 1) == 0 and wh.selective_scan_work(64, (1 << 24) + 1, 16, 1) == 0
     assert wh.expert_dispatch_work(10, 2, 0) == 0 and wh.expert_dispatch_work(-1, 2, 4) == 0
     assert wh.expert_dispatch_work(10, 2, 8) >= 0
 

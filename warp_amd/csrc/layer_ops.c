@@ -85,6 +85,7 @@ int warp_hip_short_conv(const warp_hip_conv_args *args, void *stream)
 size_t warp_hip_selective_scan_work(int tokens, int channels, int states, int n_seq, int longest)
 {
     if (tokens < 1 || channels < 1 || states < 1 || states > SCAN_MAX_STATES || n_seq < 1) return 0;
+    if (tokens > MAX_ROWS || channels > MAX_CHANNELS) return 0;
     return wk_scan_work(tokens, channels, states, n_seq, longest);
 }
 

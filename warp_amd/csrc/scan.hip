@@ -378,6 +378,16 @@ __global__ __launch_bounds__(64) void k_scan_part(scan_p p) {
     }
 }
 
+// What a chunk makes of the state h before it: exp2(l) h + e, e what it makes
+// of zero, l its decay's exponent (NaN: nothing of what was before counts, or
+// e is none either). A zero stays zero and an infinity one, as row by row, and
+// the factor goes in halves, so that a state may grow or shrink by more than
+// f32 can say at once.
+__device__ __forceinline__ float scan_over(float h, float l, float e) {
+    const float half = __builtin_fmaxf(__builtin_amdgcn_exp2f(0.5f * l), 1.17549435e-38f);
+    return l != l || h == 0.0f ? e : __builtin_fmaf(h * half, half, e);
+}
+
 // The chunks in order: end[j] becomes the state at the end of chunk j. A lane
 // takes one state, each of the block's waves a part of the chunks: first what
 // the part makes of a state of zero and how much it leaves of one, then, from
@@ -391,26 +401,26 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
     const int d = (int)(at / p.N), most = p.chunks - 1, q = (most + waves - 1) / waves;
     const int j0 = min(wave * q, most), j1 = min(j0 + q, most);
     const float A = p.A[at] * LOG2E;
-    float h = 0.0f, w = 1.0f, e[JOIN_Q], f[JOIN_Q];        // (-1: nothing of what was before is left)
+    float h = 0.0f, w = 0.0f, e[JOIN_Q], l[JOIN_Q];
     auto load = [&](int j) {
         int r[JOIN_Q];
 #pragma unroll
         for (int b = 0; b < JOIN_Q; b++)
             if (j + b < j1) {
                 e[b] = p.end[(size_t)(j + b) * dn + at];
-                f[b] = p.sum[(size_t)(j + b) * p.D + d];
+                l[b] = p.sum[(size_t)(j + b) * p.D + d];
                 r[b] = p.reset[j + b];
             }
 #pragma unroll
         for (int b = 0; b < JOIN_Q; b++)
-            if (j + b < j1) f[b] = r[b] ? -1.0f : __builtin_amdgcn_exp2f(A * f[b]);
+            if (j + b < j1) l[b] = r[b] ? __builtin_nanf("") : A * l[b];
     };
     auto walk = [&](int j, bool keep) {
 #pragma unroll
         for (int b = 0; b < JOIN_Q; b++)
             if (j + b < j1) {
-                h = f[b] < 0.0f ? e[b] : __builtin_fmaf(h, f[b], e[b]);
-                w = f[b] < 0.0f || w < 0.0f ? -1.0f : w * f[b];
+                h = scan_over(h, l[b], e[b]);
+                w += l[b];
                 if (keep && i < dn) p.end[(size_t)(j + b) * dn + at] = h;
             }
     };
@@ -423,7 +433,7 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
         left[wave][lane] = w;
         __syncthreads();
         h = 0.0f;
-        for (int v = 0; v < wave; v++) h = left[v][lane] < 0.0f ? sum[v][lane] : __builtin_fmaf(h, left[v][lane], sum[v][lane]);
+        for (int v = 0; v < wave; v++) h = scan_over(h, left[v][lane], sum[v][lane]);
     }
     if (q <= JOIN_Q) {
         walk(j0, true);
