@@ -354,7 +354,7 @@ def test_more_rows_than_a_grid_takes_at_once():
     run_scan(rng, "f32", 2, 4, [1] * 33000 + [0] * 3000 + [2] * 500, state="inplace", pad=3000)
 
 
-@pytest.mark.parametrize("T,K,E,H", [(300000, 2, 7, 4), (20, 70, 90, 33), (40, 130, 900, 9)])
+@pytest.mark.parametrize("T,K,E,H", [(300000, 2, 7, 4), (20, 70, 90, 33), (40, 130, 900, 9), (1000, 8, 256, 2070)])
 def test_dispatch_and_combine_of_many_pairs(T, K, E, H):
     rng = np.random.default_rng(T + K)
     idx = rng.integers(-1, E, size=(T, K)).astype(np.int32)

@@ -293,7 +293,7 @@ static void dispatch_launch(sort_p p, hipStream_t st) {
 extern "C" int wk_expert_dispatch(const warp_hip_dispatch_args *a, void *stream) {
     const int pairs = a->tokens * a->top_k, per = sort_per(pairs);
     sort_p p = {a->tokens, a->top_k, a->n_experts, pairs, per, (int)(((int64_t)pairs + per - 1) / per), 1, a->idx, a->offsets,
-                a->perm, a->pos, (int *)a->work, (int *)a->work + pairs, a->hidden, a->x, a->xs, a->ldx, a->ldxs};
+                a->perm, a->pos, (int *)a->work, (int *)a->work + pairs, a->x ? a->hidden : 0, a->x, a->xs, a->ldx, a->ldxs};
     while ((p.E - 1) >> p.bits) p.bits++;
     hipStream_t st = (hipStream_t)stream;
     // (rows are copied as bits)
