@@ -10,10 +10,14 @@
 // product and an exponential for the decay (the exponential issues at half
 // the rate), a product, and two fused multiply-adds, six issue slots, against
 // 8 bytes of rows per channel. The decays differ by channel and state, so
-// nothing of this is a matrix product. Single tokens are bound by their
-// states, read and written once.
+// nothing of this is a matrix product but dt' x B, an outer one over channels
+// and states: as four 4 x 4 x 1 matrix instructions a row it takes the place of
+// a fifth of the vector instructions and the same time (70 + 97 us of
+// a prompt that took 70 + 94), as each holds those up for some 15 cycles. Single
+// tokens are bound by their states, read and written once.
 
 #include <math.h>
+#include <type_traits>
 
 #include "rows.h"
 #include "warp_internal.h"
@@ -27,7 +31,6 @@ struct scan_p {
     float *sout;
     void *y;
     float *end, *sum, *init;                      // per chunk: [D][N], [D], [D][N]
-    int *reset;
 };
 
 constexpr float LOG2E = 1.44269504088896341f;
@@ -224,8 +227,9 @@ struct scan_t {
                 tb[i].e = *(const typename vec_t<T, W>::mem *)(row + (size_t)r * p.ldbc + min(n, p.N - W));
             }
         };
-        load(lo);
-        for (int t = lo; t < hi; t += U) {
+        int t = lo;
+        auto batch = [&](auto all) {
+            constexpr bool FULL = decltype(all)::value;
             float x[R], v[R], u[R], z[R], y[R];
 #pragma unroll
             for (int i = 0; i < R; i++) {
@@ -251,7 +255,7 @@ struct scan_t {
             // (one wave: what it writes to LDS is there for its next reads)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if (t + U < hi) load(t + U);
+            if (FULL) load(min(t + U, hi - 1));            // (behind the last the last again)
             if (p.softplus) {
 #pragma unroll
                 for (int i = 0; i < R; i++) v[i] = scan_softplus(v[i]);
@@ -289,39 +293,47 @@ struct scan_t {
 #pragma unroll
                 for (int i = 0; i < R; i++) {
                     const int r = i * P + (P > 1 ? own : 0);
-                    if ((n == U || r < n) && (P == LPC || part < P))
+                    if ((FULL || r < n) && (P == LPC || part < P))
                         *(T *)((char *)((T *)p.y + (size_t)(t + r) * p.ldy) + at) = (T)y[i];
                 }
             };
             if (!OUT) {
 #pragma unroll
                 for (int i = 0; i < R; i++)
-                    if (t + i * P + own < hi && part < P) sum += v[i];
+                    if ((FULL || t + i * P + own < hi) && part < P) sum += v[i];
             }
-            if (t + U <= hi) {
 #pragma unroll
-                for (int i = 0; i < U; i++) row(i);
-                if (OUT) out(U);
-            } else {
+            for (int i = 0; !FULL && i < R; i++) y[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < R; i++) y[i] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < U; i++)
-                    if (t + i < hi) row(i);
-                if (OUT) out(hi - t);
-            }
+            for (int i = 0; i < U; i++)
+                if (FULL || t + i < hi) row(i);
+            if (OUT) out(hi - t);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-        }
+        };
+        // (the last, short batch by itself: on a common way out of a loop
+        // each batch would move every state from one register to another)
+        load(lo);
+        for (; t + U <= hi; t += U) batch(std::true_type());
+        if (t < hi) batch(std::false_type());
         return scan_sum<LPC>(sum);
     }
 };
+
+// Waves to a SIMD that a batch's chunks are cut for. Of 16 states to a lane 3
+// hold the vector units 90% busy, 4 95%, and no more may share a SIMD, or some
+// get more than others. Fewer states leave room for more than their chunks are
+// cut for (5 cost more in chunks), which whole sequences use: 100 of 30 rows of
+// 4,608 channels by 16, four states a lane, 103 us, with three waves 120.
+constexpr int scan_waves(int S, int lanes) { return S == 8 || (S == 16 && lanes == 16) ? 3 : 4; }
+#define SCAN_WAVES \
+    __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(scan_waves(S, LPC), S == 16 ? scan_waves(S, LPC) : 8)))
 
 // A whole sequence per wave (chunk = 0), or the rows [j chunk, (j + 1) chunk)
 // of the packed batch, whatever sequences they hold, from the state that
 // k_scan_join found at their beginning.
 template <typename T, int S, int LPC, int U>
-__global__ __launch_bounds__(64) void k_scan_rows(scan_p p) {
+__global__ SCAN_WAVES void k_scan_rows(scan_p p) {
     __shared__ __attribute__((aligned(16))) float bc[U * 2 * S * LPC];
     scan_t<T, S, LPC, U> k;
     k.open(p);
@@ -351,11 +363,11 @@ __global__ __launch_bounds__(64) void k_scan_rows(scan_p p) {
 }
 
 // What a chunk's last sequence has at the chunk's end, from a state of zero
-// (or the sequence's first state, if it begins here: then `reset` says that
-// nothing before counts), and the sum of its dt', of which the chunk's decay
-// is the exponential. Only for a sequence that goes on in the next chunk.
+// (or the sequence's first state, if it begins here), and the sum of its dt',
+// of which the chunk's decay is the exponential (NaN if it begins here: nothing
+// before counts). Only for a sequence that goes on in the next chunk.
 template <typename T, int S, int LPC, int U>
-__global__ __launch_bounds__(64) void k_scan_part(scan_p p) {
+__global__ SCAN_WAVES void k_scan_part(scan_p p) {
     __shared__ __attribute__((aligned(16))) float bc[U * S * LPC];
     scan_t<T, S, LPC, U> k;
     k.open(p);
@@ -373,8 +385,7 @@ __global__ __launch_bounds__(64) void k_scan_part(scan_p p) {
         if (from) k.store(p, p.init + (size_t)j * dn);
         const float sum = k.template rows<false>(p, max(q.b, r0), r1, bc);
         k.store(p, p.end + (size_t)j * dn);
-        if (k.part == 0) p.sum[(size_t)j * p.D + k.d] = sum;
-        if (blockIdx.x == 0 && k.lane == 0) p.reset[j] = begins;
+        if (k.part == 0) p.sum[(size_t)j * p.D + k.d] = begins ? __builtin_nanf("") : sum;
     }
 }
 
@@ -393,36 +404,37 @@ __device__ __forceinline__ float scan_over(float h, float l, float e) {
 // the part makes of a state of zero and how much it leaves of one, then, from
 // the state that the parts before it leave, the states themselves. Up to
 // JOIN_Q chunks of a part stay in registers between the two.
-constexpr int JOIN_Q = 12, JOIN_W = 16;
-__global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
+constexpr int JOIN_Q = 10, JOIN_W = 16;
+__global__ __launch_bounds__(64 * JOIN_W, 8) void k_scan_join(scan_p p) {
     __shared__ float sum[JOIN_W][64], left[JOIN_W][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const size_t dn = (size_t)p.D * p.N, i = (size_t)blockIdx.x * 64 + lane, at = min(i, dn - 1);
-    const int d = (int)(at / p.N), most = p.chunks - 1, q = (most + waves - 1) / waves;
+    const size_t dn = (size_t)p.D * p.N;                   // (at most 2^32: any state's index fits)
+    const unsigned i = blockIdx.x * 64 + lane, at = min(i, (unsigned)(dn - 1));
+    const int d = (int)(at / (unsigned)p.N), most = p.chunks - 1, q = (most + waves - 1) / waves;
     const int j0 = min(wave * q, most), j1 = min(j0 + q, most);
     const float A = p.A[at] * LOG2E;
     float h = 0.0f, w = 0.0f, e[JOIN_Q], l[JOIN_Q];
+    // (behind the part's last chunk: ones that leave a state as it is)
     auto load = [&](int j) {
-        int r[JOIN_Q];
 #pragma unroll
-        for (int b = 0; b < JOIN_Q; b++)
-            if (j + b < j1) {
-                e[b] = p.end[(size_t)(j + b) * dn + at];
-                l[b] = p.sum[(size_t)(j + b) * p.D + d];
-                r[b] = p.reset[j + b];
-            }
+        for (int b = 0; b < JOIN_Q; b++) {
+            const int c = min(j + b, most - 1);
+            e[b] = p.end[(size_t)c * dn + at];
+            l[b] = p.sum[(size_t)c * p.D + d];
+        }
 #pragma unroll
-        for (int b = 0; b < JOIN_Q; b++)
-            if (j + b < j1) l[b] = r[b] ? __builtin_nanf("") : A * l[b];
+        for (int b = 0; b < JOIN_Q; b++) {
+            e[b] = j + b < j1 ? e[b] : 0.0f;
+            l[b] = j + b < j1 ? A * l[b] : 0.0f;
+        }
     };
     auto walk = [&](int j, bool keep) {
 #pragma unroll
-        for (int b = 0; b < JOIN_Q; b++)
-            if (j + b < j1) {
-                h = scan_over(h, l[b], e[b]);
-                w += l[b];
-                if (keep && i < dn) p.end[(size_t)(j + b) * dn + at] = h;
-            }
+        for (int b = 0; b < JOIN_Q; b++) {
+            h = scan_over(h, l[b], e[b]);
+            w += l[b];
+            if (keep && j + b < j1 && i < dn) p.end[(size_t)(j + b) * dn + at] = h;
+        }
     };
     for (int j = j0; j < j1; j += JOIN_Q) {
         load(j);
@@ -456,8 +468,8 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_scan_join(scan_p p) {
 // as many waves as keep the SIMDs busy (`rows`, and `part` for the chunks'
 // first pass), and what the launches take. One bf16 prompt of 4,608 channels
 // and 16 states: 4,096 rows take 1,840 us in one piece, 609 with 4 states a
-// lane, 173 in 41 chunks (70 + 9 + 94), 400 rows 176, 63 and 38. 1,999 f32 rows
-// of 2,304 channels and 64 states in 13 sequences: 145 in chunks (57 + 8 + 80)
+// lane, 165 in 54 chunks (65 + 11 + 89), 400 rows 176, 63 and 38. 1,999 f32 rows
+// of 2,304 channels and 64 states in 13 sequences: 136 in chunks (53 + 10 + 73)
 // or, as their lengths are more or less even, 120 to 187 a wave to a sequence.
 struct scan_plan {
     int S, lanes, chunk, chunks;
@@ -469,13 +481,16 @@ static scan_plan scan_try(int S, int lanes, int tokens, int D, int n_seq, int lo
     // (a sequence longer than the others runs on by itself)
     const double over = longest - (double)tokens / n_seq;
     scan_plan r = {S, lanes, 0, 0, fmax(5000 + alone * longest, rows * load + alone * fmax(over, 0))};
-    double most = (S == 16 ? 3 : S == 8 ? 4 : 5) * simds / waves;        // as many to a SIMD as registers allow
-    if (most > tokens / 16) most = tokens / 16;
-    if (most < 2) return r;
-    // (a chunk more than fits would run by itself at the end)
-    const int chunk = ((tokens + (int)most - 1) / (int)most + 3) / 4 * 4, chunks = (tokens + chunk - 1) / chunk;
-    const double ns = 8000 + fmax(8000 + alone * chunk, rows * load) + fmax(8000 + 0.75 * alone * chunk, part * load);
-    if (chunks >= 2 && ns < r.ns) r = {S, lanes, chunk, chunks, ns};
+    // as many chunks as there are waves for, or as k_scan_join joins in one go
+    const int once = JOIN_Q * JOIN_W + 1, fit = (int)fmin(scan_waves(S, lanes) * simds / waves, tokens / 16);
+    for (int most : {fit, once}) {
+        if (most < 2 || most > fit) continue;
+        // (one more than fits would run by itself at the end)
+        const int chunk = ((tokens + most - 1) / most + 3) / 4 * 4, chunks = (tokens + chunk - 1) / chunk;
+        const double join = 4000 + 0.0016 * chunks * D * S * lanes + (chunks > once ? 8000 : 0);
+        const double ns = 4000 + join + fmax(8000 + alone * chunk, rows * load) + fmax(8000 + 0.75 * alone * chunk, part * load);
+        if (chunks >= 2 && ns < r.ns) r = {S, lanes, chunk, chunks, ns};
+    }
     return r;
 }
 static scan_plan scan_split(int tokens, int D, int N, int n_seq, int longest) {
@@ -489,7 +504,7 @@ static scan_plan scan_split(int tokens, int D, int N, int n_seq, int longest) {
     return few.ns < many.ns ? few : many;
 }
 static size_t scan_floats(const scan_plan &s, int D, int N) {
-    return s.chunk ? (size_t)s.chunks * (2 * (size_t)D * N + D + 1) : 0;
+    return s.chunk ? (size_t)s.chunks * (2 * (size_t)D * N + D) : 0;
 }
 
 template <typename T, int S, int LPC, int U>
@@ -553,7 +568,7 @@ extern "C" int wk_selective_scan(const warp_hip_scan_args *a, void *stream) {
     scan_p p = {a->tokens, a->n_seq, a->channels, a->states, a->groups, a->n_slots, a->softplus, s.chunk, s.chunks,
                 a->starts, a->slots, a->x, a->dt, a->B, a->C, a->z, a->ldx, a->lddt, a->ldbc, a->ldz, a->ldy,
                 a->A, a->D, a->dt_bias, a->state_in, a->state_out, a->y,
-                w, w + 2 * s.chunks * dn, w + s.chunks * dn, (int *)(w + s.chunks * (2 * dn + a->channels))};
+                w, w + 2 * s.chunks * dn, w + s.chunks * dn};
     if (a->type == WARP_HIP_F32) scan_launch<float>(p, s, (hipStream_t)stream);
     else if (a->type == WARP_HIP_BF16) scan_launch<bf16_t>(p, s, (hipStream_t)stream);
     else scan_launch<f16_t>(p, s, (hipStream_t)stream);
