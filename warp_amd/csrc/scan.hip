@@ -126,6 +126,17 @@ __device__ __forceinline__ float scan_from(float v, int p) {
 #undef DPP
 }
 
+// A lane's element `at` bytes into a row. ONE: the row is the wave's, its
+// address stays in scalar registers and the lane's offset is the load's own
+// (left to itself, the compiler adds the two in each lane).
+template <bool ONE, typename T>
+__device__ __forceinline__ __attribute__((address_space(1))) T *scan_at(const char *row, unsigned at) {
+    typedef __attribute__((address_space(1))) char *bytes;
+    bytes b = (bytes)(char *)row;
+    if (ONE) asm volatile("" : "+s"(b));
+    return (__attribute__((address_space(1))) T *)(b + at);
+}
+
 // Prompts. LPC lanes of a wave share a channel, S states each in registers;
 // a wave is a block and takes 64 / LPC channels of one group. The rows go in
 // batches of U: their B and C are laid out in LDS as f32, where a row's lie at
@@ -209,15 +220,59 @@ struct scan_t {
         T tx[R], td[R], tz[R];
         vec_t<T, W> tb[M];
         float sum = 0.0f;
-        const unsigned at = d * sizeof(T);
+        // this lane's offset in a row (anew each time, or the additions to it would leave their loads)
+        auto mine = [&] {
+            unsigned at = d * sizeof(T);
+            if (P == 1) asm volatile("" : "+v"(at));
+            return at;
+        };
         const int own = part % P;                          // this lane's rows: own, own + P, ...
+        const void *gate = p.z ? p.z : p.x;                // (without one x again, which saves the loads a branch each)
+        const size_t sx = p.ldx * sizeof(T), sd = p.lddt * sizeof(T), sz = p.z ? p.ldz * sizeof(T) : sx, sy = p.ldy * sizeof(T);
+        // With one row a batch to a lane, where it and the lane's parts of B and C lie behind the batch's first
+        // row is multiplied out once, for full batches: a product of 64 bits costs as much as three states
+        // (1,999 f32 rows of 2,304 channels and 64 states 130 -> 125 us; lanes with two rows gain nothing).
+        constexpr bool ONCE = P > 1 && R == 1;
+        size_t wx, wd, wz, wb[M];
+        auto reach = [&](int rows) {
+            const size_t r = min(own, rows - 1);
+            wx = r * sx, wd = r * sd, wz = r * sz;
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+                const int e = (lane + 64 * i) * W;
+                wb[i] = (size_t)min(e / (RS * K), rows - 1) * p.ldbc + (size_t)g * p.N + min(e % RS, p.N - W);
+            }
+        };
         auto load = [&](int t) {
+            if constexpr (ONCE) {
+                if (t + U > hi) reach(hi - t);             // (which is the last)
+                tx[0] = *(const T *)((const char *)p.x + t * sx + wx + d * sizeof(T));
+                td[0] = *(const T *)((const char *)p.dt + t * sd + wd + d * sizeof(T));
+                if (OUT) tz[0] = *(const T *)((const char *)gate + t * sz + wz + d * sizeof(T));
+#pragma unroll
+                for (int i = 0; i < M; i++) {
+                    const T *row = (const T *)(OUT && (lane + 64 * i) * W / RS % K ? p.C : p.B) + t * p.ldbc;
+                    tb[i].e = *(const typename vec_t<T, W>::mem *)(row + wb[i]);
+                }
+                return;
+            }
+            const unsigned at = mine();
+            size_t r = min(t + (P > 1 ? own : 0), hi - 1);
+            const char *xr = (const char *)p.x + r * sx, *dr = (const char *)p.dt + r * sd, *zr = (const char *)gate + r * sz;
 #pragma unroll
             for (int i = 0; i < R; i++) {
-                const size_t r = min(t + i * P + (P > 1 ? own : 0), hi - 1);
-                tx[i] = *(const T *)((const char *)((const T *)p.x + r * p.ldx) + at);
-                td[i] = *(const T *)((const char *)((const T *)p.dt + r * p.lddt) + at);
-                if (OUT && p.z) tz[i] = *(const T *)((const char *)((const T *)p.z + r * p.ldz) + at);
+                tx[i] = *scan_at<P == 1, const T>(xr, at);
+                td[i] = *scan_at<P == 1, const T>(dr, at);
+                if (OUT) tz[i] = *scan_at<P == 1, const T>(zr, at);
+                const bool on = t + (i + 1) * P + (P > 1 ? own : 0) < hi;      // (behind the last the last again)
+                if (P == 1) {
+                    xr += on ? sx : 0;
+                    dr += on ? sd : 0;
+                    zr += on ? sz : 0;
+                } else {
+                    r = min(t + (i + 1) * P + own, hi - 1);
+                    xr = (const char *)p.x + r * sx, dr = (const char *)p.dt + r * sd, zr = (const char *)gate + r * sz;
+                }
             }
 #pragma unroll
             for (int i = 0; i < M; i++) {
@@ -235,7 +290,7 @@ struct scan_t {
             for (int i = 0; i < R; i++) {
                 x[i] = (float)tx[i];
                 v[i] = (float)td[i] + bias;
-                if (OUT && p.z) z[i] = (float)tz[i];
+                if (OUT) z[i] = (float)tz[i];
             }
 #pragma unroll
             for (int i = 0; i < M; i++) {
@@ -255,7 +310,7 @@ struct scan_t {
             // (one wave: what it writes to LDS is there for its next reads)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if (FULL) load(min(t + U, hi - 1));            // (behind the last the last again)
+            if (FULL) load(min(t + U, hi - 1));
             if (p.softplus) {
 #pragma unroll
                 for (int i = 0; i < R; i++) v[i] = scan_softplus(v[i]);
@@ -290,12 +345,11 @@ struct scan_t {
 #pragma unroll
                     for (int i = 0; i < R; i++) y[i] *= rows_silu(z[i]);
                 }
+                const unsigned at = mine();
+                char *to = (char *)p.y + (size_t)(t + (P > 1 ? own : 0)) * sy;
 #pragma unroll
-                for (int i = 0; i < R; i++) {
-                    const int r = i * P + (P > 1 ? own : 0);
-                    if ((FULL || r < n) && (P == LPC || part < P))
-                        *(T *)((char *)((T *)p.y + (size_t)(t + r) * p.ldy) + at) = (T)y[i];
-                }
+                for (int i = 0; i < R; i++, to += P * sy)
+                    if ((FULL || i * P + (P > 1 ? own : 0) < n) && (P == LPC || part < P)) *scan_at<P == 1, T>(to, at) = (T)y[i];
             };
             if (!OUT) {
 #pragma unroll
@@ -313,6 +367,7 @@ struct scan_t {
         };
         // (the last, short batch by itself: on a common way out of a loop
         // each batch would move every state from one register to another)
+        if constexpr (ONCE) reach(U);
         load(lo);
         for (; t + U <= hi; t += U) batch(std::true_type());
         if (t < hi) batch(std::false_type());
@@ -325,7 +380,7 @@ struct scan_t {
 // get more than others. Fewer states leave room for more than their chunks are
 // cut for (5 cost more in chunks), which whole sequences use: 100 of 30 rows of
 // 4,608 channels by 16, four states a lane, 103 us, with three waves 120.
-constexpr int scan_waves(int S, int lanes) { return S == 8 || (S == 16 && lanes == 16) ? 3 : 4; }
+constexpr int scan_waves(int S, int lanes) { return S == 8 || (S == 16 && lanes >= 8) ? 3 : 4; }
 #define SCAN_WAVES \
     __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(scan_waves(S, LPC), S == 16 ? scan_waves(S, LPC) : 8)))
 
