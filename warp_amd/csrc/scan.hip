@@ -523,8 +523,8 @@ __global__ __launch_bounds__(64 * JOIN_W, 8) void k_scan_join(scan_p p) {
 // as many waves as keep the SIMDs busy (`rows`, and `part` for the chunks'
 // first pass), and what the launches take. One bf16 prompt of 4,608 channels
 // and 16 states: 4,096 rows take 1,840 us in one piece, 609 with 4 states a
-// lane, 165 in 54 chunks (65 + 11 + 89), 400 rows 176, 63 and 38. 1,999 f32 rows
-// of 2,304 channels and 64 states in 13 sequences: 136 in chunks (53 + 10 + 73)
+// lane, 164 in 54 chunks (66 + 11 + 87), 400 rows 176, 63 and 38. 1,999 f32 rows
+// of 2,304 channels and 64 states in 13 sequences: 137 in chunks (53 + 10 + 74)
 // or, as their lengths are more or less even, 120 to 187 a wave to a sequence.
 struct scan_plan {
     int S, lanes, chunk, chunks;
